@@ -48,7 +48,8 @@ extern "C" {
 #define SWARP_MAX_CTA_AGENTS 1024
 #define SWARP_NUM_PARAMS 22
 
-typedef enum { SWARP_F32 = 0, SWARP_F64 = 1 } swarp_dtype_t;
+/* worlds take SWARP_F32 and SWARP_F64; the 16-bit types are those of the policy operators */
+typedef enum { SWARP_F32 = 0, SWARP_F64 = 1, SWARP_BF16 = 2, SWARP_F16 = 3 } swarp_dtype_t;
 typedef enum { SWARP_BOUNDS_NONE = 0, SWARP_BOUNDS_SOFT = 1, SWARP_BOUNDS_CLAMP = 2 } swarp_bounds_t;
 
 /* The five live 2-D agent fields, structure of arrays. For a state at one time the
@@ -217,6 +218,145 @@ int swarp_rollout_noalloc(const swarp_world_t* w, int32_t horizon, swarp_state_t
  * against the kernels env chunk by env chunk. */
 int swarp_copy_rows(void* dst, size_t dst_pitch, const void* src, size_t src_pitch,
                     size_t row_bytes, size_t rows, void* stream);
+
+/* ---- Policy training: what a trainer runs on the rollouts ---------------------------
+ * Advantages of a rollout, the clipped policy loss with its gradient, and the AdamW step.
+ * None of them has a counterpart on the reference's step path (its trainer forms them in
+ * torch). All launch on `stream`, allocate nothing and are deterministic: the same inputs
+ * give the same bits. */
+
+/* A batch of rows, each a categorical distribution over `vocab` tokens given by logits, and
+ * the token taken in each row. With lp the log probability of the row's token, r =
+ * exp(lp - old_logp), A its advantage, d = ref_logp - lp and H the row's entropy:
+ *   row loss = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+ *              + kl_coef (e^d - d - 1) - entropy_coef H
+ * and the loss is its mean over the rows that mask admits (mean != 0) or its sum. A row
+ * that mask leaves out is not read: its logp and entropy are 0 and its gradient is 0. A
+ * logit of -inf is a token of probability 0; a row of nothing else has logp -inf, entropy 0
+ * and no loss or gradient (it still counts). A token outside [0, vocab) gives NaN. With no
+ * row admitted the loss is 0. */
+typedef struct {
+  int32_t dtype;           /* of logits and grad: SWARP_F32, SWARP_BF16 or SWARP_F16 */
+  int32_t tokens_64;       /* tokens are int64 (else int32) */
+  int64_t rows, vocab;     /* >= 0, >= 1 */
+  /* row i of logits starts at (i / inner) * stride_outer + (i % inner) * stride_inner
+   * elements; its vocab elements are adjacent */
+  int64_t inner, stride_outer, stride_inner;
+  const void* logits;
+  const void* tokens;      /* [rows] */
+  const float* old_logp;   /* [rows] */
+  const float* advantages; /* [rows] */
+  const float* ref_logp;   /* [rows] or NULL (no KL term) */
+  const uint8_t* mask;     /* [rows], 0 = left out; or NULL */
+  float clip_low, clip_high, kl_coef, entropy_coef;
+  int32_t mean;
+  float grad_scale;        /* grad is that of grad_scale * loss */
+  float* logp;             /* out [rows] */
+  float* entropy;          /* out [rows] */
+  float* loss;             /* out [1] */
+  float* stats;            /* out [4]: the mean (or sum) over the admitted rows of the clipped
+                              term, e^d - d - 1, H and (1 where the clip cut) */
+  void* grad;              /* out [rows, vocab] contiguous, or NULL */
+} swarp_policy_t;
+
+/* Bytes of device workspace of one swarp_policy_loss or swarp_policy_grad call (0 for an
+ * invalid batch). */
+size_t swarp_policy_workspace_bytes(const swarp_policy_t* p);
+
+/* The loss, and with `grad` its gradient in the same pass over the logits. */
+int swarp_policy_loss(const swarp_policy_t* p, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* The gradient alone, of cotangent[0] * grad_scale * loss (cotangent: one float on the
+ * device). With skip_unit the call writes nothing when cotangent[0] is 1: `grad` then
+ * holds the gradient that swarp_policy_loss left there. logp, entropy, loss and stats are
+ * not used. */
+int swarp_policy_grad(const swarp_policy_t* p, const float* cotangent, int32_t skip_unit,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* Log probabilities of the tokens and entropies alone: rows, vocab, strides, logits,
+ * tokens, logp and entropy are used. */
+int swarp_token_logp(const swarp_policy_t* p, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+/* Generalised advantage estimates of a rollout of `steps` steps over `columns` agents:
+ *   A_t = r_t + gamma V'_t - V_t + gamma lambda A_{t+1},  returns_t = A_t + V_t
+ * V'_t is next_values[t], or without it values[t + 1] (last_values after the last step); it
+ * is dropped, whatever it holds, where terminated[t]. A_{t+1} is dropped where
+ * terminated[t] or truncated[t]. rewards, values, next_values, advantages, returns
+ * [steps, columns] and last_values [columns] are SWARP_F32 or SWARP_F64; terminated and
+ * truncated are [steps, columns / columns_per_flag] bytes, or NULL. */
+typedef struct {
+  int32_t dtype;
+  int32_t columns_per_flag; /* >= 1, divides columns */
+  int64_t steps, columns;   /* >= 0 */
+  const void* rewards;
+  const void* values;
+  const void* next_values; /* or NULL */
+  const void* last_values; /* or NULL where next_values is given */
+  const uint8_t* terminated;
+  const uint8_t* truncated;
+  double gamma, lambda;
+  void* advantages;
+  void* returns;
+} swarp_gae_t;
+
+size_t swarp_gae_workspace_bytes(const swarp_gae_t* g);
+int swarp_gae(const swarp_gae_t* g, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One parameter tensor of `n` contiguous elements and its AdamW state. */
+typedef struct {
+  int64_t n;
+  void* param;          /* swarp_adamw_t.dtype, updated */
+  const void* grad;     /* the same dtype */
+  float* master;        /* the parameter in 32 bits, updated; required for 16-bit dtypes
+                           (param is then its rounding), NULL for SWARP_F32 */
+  void* exp_avg;        /* float [n], or with 8-bit moments bytes [n] */
+  void* exp_avg_sq;
+  uint8_t* exp_avg_exp; /* 8-bit moments: one exponent per SWARP_MOMENT_BLOCK elements */
+  uint8_t* exp_avg_sq_exp;
+} swarp_adamw_tensor_t;
+
+/* 8-bit moments are kept in blocks of SWARP_MOMENT_BLOCK elements that share one exponent
+ * E, the float32 exponent field of the block's largest magnitude. With q(x) = (bits(|x|) +
+ * (R << 4)) >> 20, that is the exponent and three mantissa bits of x rounded up or down at
+ * random by the 16 random bits R, the first moment is a sign bit and seven bits f = q -
+ * (8 E - 112), zero below f = 8, and the second moment eight bits q - (8 E - 247), at
+ * least 1 where it is not zero. R is a hash of (seed, step, tensor index, element): the
+ * low half word for the first moment, the high for the second. */
+#define SWARP_MOMENT_BLOCK 256
+
+typedef struct {
+  int32_t dtype;        /* of param and grad: SWARP_F32, SWARP_BF16 or SWARP_F16 */
+  int32_t moment_bits;  /* 32 or 8 */
+  int64_t step;         /* counted from 1 */
+  double lr, beta1, beta2, eps, weight_decay;
+  uint32_t seed;        /* of the 8-bit rounding */
+  uint32_t first_tensor; /* index of tensors[0] in the rounding's hash */
+  /* clipping: gradients are scaled by min(1, max_norm / (norm + 1e-6)) with norm the root
+   * of the sum of `norm_partials`; NULL = no clipping */
+  const double* norm_partials;
+  int64_t n_norm_partials;
+  double max_norm;
+  float* grad_norm;     /* out: one float, the norm; or NULL */
+} swarp_adamw_t;
+
+/* Number of doubles that swarp_grad_norm_partials writes for n_tensors tensors. */
+int64_t swarp_grad_norm_partials_count(int64_t n_tensors);
+
+/* Sums of squares of the gradients (n and grad of each entry are used), one per CTA. */
+int swarp_grad_norm_partials(int32_t dtype, const swarp_adamw_tensor_t* tensors,
+                             int64_t n_tensors, double* partials, void* stream);
+
+/* One decoupled-weight-decay Adam step over all tensors (host array):
+ *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+ *   p = p (1 - lr wd) - lr / (1 - b1^step) * m / (sqrt(v / (1 - b2^step)) + eps) */
+int swarp_adamw_step(const swarp_adamw_t* opt, const swarp_adamw_tensor_t* tensors,
+                     int64_t n_tensors, void* stream);
+
+/* The values that n 8-bit moments stand for, as SWARP_F32 or SWARP_BF16 (both exact). */
+int swarp_moment8_values(const uint8_t* codes, const uint8_t* exponents, int64_t n,
+                         int32_t is_signed, int32_t dtype, void* out, void* stream);
 
 /* Static description of a return code. */
 const char* swarp_error_string(int code);

@@ -55,6 +55,16 @@ from swarp_b200.interop.autograd import (
 from swarp_b200.core.sharding import PairReducer, env_shard, reduce_loss_and_grad_norm
 from swarp_b200.interop.compile import compiled_warp_step, register_stepper
 from swarp_b200.interop.graphs import GraphedRollout
+from swarp_b200.learn import (
+    AdamW,
+    Moment8,
+    PolicyLoss,
+    adamw_step,
+    gae,
+    policy_loss,
+    policy_loss_and_grad,
+    token_logp,
+)
 from swarp_b200.scenarios import SCENARIOS, NavigationScenario, make_scenario, scenario_class
 
 __version__ = "0.1.0"
@@ -84,7 +94,8 @@ def make(name: str, n_envs: int, **kwargs) -> Environment:
 
 
 __all__ = [
-    "AgentConfig", "AgentShape", "BodyState", "ControlMode", "DynamicsModel", "Environment",
+    "AdamW", "Moment8", "PolicyLoss", "adamw_step", "gae", "policy_loss",
+    "policy_loss_and_grad", "token_logp", "AgentConfig", "AgentShape", "BodyState", "ControlMode", "DynamicsModel", "Environment",
     "GradRing", "GraphedRollout", "PairReducer", "compiled_warp_step", "env_shard",
     "reduce_loss_and_grad_norm", "register_stepper", "Integrator", "NUM_PARAMS", "NavigationScenario", "ObstacleKind", "ObstacleShape",
     "Obstacles", "PARAM_FIELDS", "P_HALF_X", "P_HALF_Y", "P_LF", "P_LR", "P_MASS", "P_MAX_ACCEL",

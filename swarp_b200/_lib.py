@@ -76,6 +76,50 @@ class WorldC(C.Structure):
     ]
 
 
+class Policy(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("tokens_64", C.c_int32),
+        ("rows", C.c_int64), ("vocab", C.c_int64),
+        ("inner", C.c_int64), ("stride_outer", C.c_int64), ("stride_inner", C.c_int64),
+        ("logits", C.c_void_p), ("tokens", C.c_void_p), ("old_logp", C.c_void_p),
+        ("advantages", C.c_void_p), ("ref_logp", C.c_void_p), ("mask", C.c_void_p),
+        ("clip_low", C.c_float), ("clip_high", C.c_float),
+        ("kl_coef", C.c_float), ("entropy_coef", C.c_float),
+        ("mean", C.c_int32), ("grad_scale", C.c_float),
+        ("logp", C.c_void_p), ("entropy", C.c_void_p), ("loss", C.c_void_p),
+        ("stats", C.c_void_p), ("grad", C.c_void_p),
+    ]
+
+
+class Gae(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("columns_per_flag", C.c_int32),
+        ("steps", C.c_int64), ("columns", C.c_int64),
+        ("rewards", C.c_void_p), ("values", C.c_void_p), ("next_values", C.c_void_p),
+        ("last_values", C.c_void_p), ("terminated", C.c_void_p), ("truncated", C.c_void_p),
+        ("gamma", C.c_double), ("lambda_", C.c_double),
+        ("advantages", C.c_void_p), ("returns", C.c_void_p),
+    ]
+
+
+class AdamWTensor(C.Structure):
+    _fields_ = [
+        ("n", C.c_int64), ("param", C.c_void_p), ("grad", C.c_void_p), ("master", C.c_void_p),
+        ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
+        ("exp_avg_exp", C.c_void_p), ("exp_avg_sq_exp", C.c_void_p),
+    ]
+
+
+class AdamWOpt(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("moment_bits", C.c_int32), ("step", C.c_int64),
+        ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+        ("weight_decay", C.c_double), ("seed", C.c_uint32), ("first_tensor", C.c_uint32),
+        ("norm_partials", C.c_void_p), ("n_norm_partials", C.c_int64), ("max_norm", C.c_double),
+        ("grad_norm", C.c_void_p),
+    ]
+
+
 #: exported symbol -> (restype, argtypes); every entry point the header declares
 SIGNATURES = {
     "swarp_rollout_workspace_bytes": (C.c_size_t, [C.POINTER(WorldC), C.c_int32]),
@@ -91,6 +135,19 @@ SIGNATURES = {
                                         State, State, State, C.c_void_p, State, C.c_void_p]),
     "swarp_copy_rows": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_size_t,
                                   C.c_size_t, C.c_void_p]),
+    "swarp_policy_workspace_bytes": (C.c_size_t, [C.POINTER(Policy)]),
+    "swarp_policy_loss": (C.c_int, [C.POINTER(Policy), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "swarp_policy_grad": (C.c_int, [C.POINTER(Policy), C.c_void_p, C.c_int32, C.c_void_p,
+                                    C.c_size_t, C.c_void_p]),
+    "swarp_token_logp": (C.c_int, [C.POINTER(Policy), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "swarp_gae_workspace_bytes": (C.c_size_t, [C.POINTER(Gae)]),
+    "swarp_gae": (C.c_int, [C.POINTER(Gae), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "swarp_grad_norm_partials_count": (C.c_int64, [C.c_int64]),
+    "swarp_grad_norm_partials": (C.c_int, [C.c_int32, C.c_void_p, C.c_int64, C.c_void_p,
+                                           C.c_void_p]),
+    "swarp_adamw_step": (C.c_int, [C.POINTER(AdamWOpt), C.c_void_p, C.c_int64, C.c_void_p]),
+    "swarp_moment8_values": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32,
+                                       C.c_void_p, C.c_void_p]),
     "swarp_error_string": (C.c_char_p, [C.c_int]),
     "swarp_abi_version": (C.c_int32, []),
 }

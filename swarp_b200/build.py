@@ -22,13 +22,17 @@ SOURCES = ["capi.cu", "noalloc.cu", "k_fwd_f32.cu", "k_fwd_f64.cu", "k_bwd_f32.c
            "k_bwd_f32_box.cu", "k_bwd_f64_box.cu", "k_fwd_f32_drone.cu", "k_fwd_f64_drone.cu",
            "k_bwd_f32_drone.cu", "k_bwd_f64_drone.cu", "k_cl_fwd_f32.cu", "k_cl_fwd_f64.cu",
            "k_cl_bwd_f32.cu", "k_cl_bwd_f64.cu"]
+# the policy-training operators: no common headers, and flags of their own
+LEARN_SOURCES = ["learn_policy.cu", "learn_gae.cu", "learn_adamw.cu"]
 # headers every translation unit includes, and those only some include
 COMMON_HEADERS = ["launch.cuh", "rollout.cuh", "physics.cuh", "bodies.cuh", "boxes.cuh",
                   "boxes_vjp.cuh", "drone.cuh"]
 EXTRA_HEADERS = {"k_x2_f32.cu": ["rollout_x2.cuh"], "capi.cu": ["rollout_cluster.cuh"],
                  **{f"k_cl_{d}_{t}.cu": ["k_cl.cuh", "rollout_cluster.cuh"]
-                    for d in ("fwd", "bwd") for t in ("f32", "f64")}}
-DEPS = [*SOURCES, *COMMON_HEADERS, "rollout_x2.cuh", "k_cl.cuh", "rollout_cluster.cuh"]
+                    for d in ("fwd", "bwd") for t in ("f32", "f64")},
+                 **{s: ["learn.cuh"] for s in LEARN_SOURCES}}
+DEPS = [*SOURCES, *LEARN_SOURCES, *COMMON_HEADERS, "rollout_x2.cuh", "k_cl.cuh", "rollout_cluster.cuh",
+        "learn.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # -ftz=true: float32 arithmetic flushes subnormal inputs and results to zero (float64 is
 # unaffected); every float kernel is built the same way, so the kernels that must agree bit
@@ -36,6 +40,10 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # still do
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "--extended-lambda", "-fmad=false", "-ftz=true",
          "-Xcompiler", "-fPIC", "-Xcompiler", "-O2"]
+# the learn_* kernels compile with subnormals kept, since second moments of small gradients
+# are subnormal, and with contraction left to the compiler except where a kernel writes a
+# rounding out (8-bit moments)
+LEARN_FLAGS = [f for f in FLAGS if f not in ("-fmad=false", "-ftz=true")]
 LINK = ["--shared", "-cudart", "shared"]
 
 
@@ -68,15 +76,18 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
     headers.append(os.path.join(ROOT, "include", "swarp_b200.h"))
     headers.append(os.path.abspath(__file__))
     newest_hdr = max(os.path.getmtime(h) for h in headers)
-    for src in SOURCES:
+    newest_learn = max(os.path.getmtime(h) for h in headers[-2:])  # the ABI header, this file
+    for src in [*SOURCES, *LEARN_SOURCES]:
+        learn = src in LEARN_SOURCES
         obj = os.path.join(objdir, src.replace(".cu", ".o"))
         objs.append(obj)
         path = os.path.join(CSRC, src)
         own = [os.path.getmtime(os.path.join(CSRC, h)) for h in EXTRA_HEADERS.get(src, [])]
         if (not force and not extra and os.path.exists(obj)
-                and os.path.getmtime(obj) > max(newest_hdr, os.path.getmtime(path), *own)):
+                and os.path.getmtime(obj) > max(newest_learn if learn else newest_hdr,
+                                                os.path.getmtime(path), *own)):
             continue
-        cmd = [nvcc(), *ARCH, *FLAGS, *(extra or []), "-c", "-o", obj, path]
+        cmd = [nvcc(), *ARCH, *(LEARN_FLAGS if learn else FLAGS), *(extra or []), "-c", "-o", obj, path]
         if verbose:
             print(" ".join(cmd), flush=True)
         procs.append(subprocess.Popen(cmd))
