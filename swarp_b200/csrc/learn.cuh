@@ -31,6 +31,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// 2^x to 2 ulp; what is below 2^-126 becomes 0
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 template <typename V> __device__ __forceinline__ V warp_sum(V v) {
 #pragma unroll
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(kAll, v, d);
