@@ -16,23 +16,157 @@ template <typename T> struct Args {
   T gamma, decay;  // gamma lambda
 };
 
-// One thread per column walks the steps backwards.
+template <typename T> struct Step {
+  T r = 0, v = 0, next = 0;  // next: V' where next_values are given
+  bool term = false, stop = false;
+};
+template <typename T>
+__device__ __forceinline__ Step<T> load_step(const Args<T>& a, long long t, long long j,
+                                             long long f) {
+  const long long k = t * a.columns + j, g = t * a.flags + f;
+  Step<T> s;
+  s.r = a.r[k];
+  s.v = a.v[k];
+  s.next = a.next ? a.next[k] : T(0);
+  s.term = a.term && a.term[g];
+  // with no decay at all the next step's advantage is out, whatever it is
+  s.stop = s.term || (a.trunc && a.trunc[g]) || a.decay == T(0);
+  return s;
+}
+
+// ------------------------------------------------------------------ many columns
+// One thread per column walks the steps backwards, kAhead steps' loads in flight.
 template <typename T> __global__ void __launch_bounds__(256) gae_columns_kernel(Args<T> a) {
+  constexpr int kAhead = 8;
   const long long j = blockIdx.x * 256ll + threadIdx.x;
   if (j >= a.columns) return;
   const long long f = j / a.per_flag;
   T A = 0, after = a.next ? T(0) : a.last[j];
-  for (long long t = a.steps - 1; t >= 0; --t) {
-    const long long k = t * a.columns + j;
-    const bool term = a.term && a.term[t * a.flags + f];
-    const bool stop = term || (a.trunc && a.trunc[t * a.flags + f]);
-    const T v = a.v[k], follow = a.next ? a.next[k] : after;
-    const T d = a.r[k] + (term ? T(0) : a.gamma * follow) - v;
-    A = stop ? d : d + a.decay * A;
-    a.adv[k] = A;
-    a.ret[k] = A + v;
-    after = v;
+  for (long long t = a.steps; t > 0; t -= kAhead) {
+    Step<T> s[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (t - 1 - k >= 0) s[k] = load_step(a, t - 1 - k, j, f);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (t - 1 - k < 0) break;
+      const T d = s[k].r + (s[k].term ? T(0) : a.gamma * (a.next ? s[k].next : after)) - s[k].v;
+      A = s[k].stop ? d : d + a.decay * A;
+      const long long at = (t - 1 - k) * a.columns + j;
+      a.adv[at] = A;
+      a.ret[at] = A + s[k].v;
+      after = s[k].v;
+    }
   }
+}
+
+// ------------------------------------------------------------------- few columns
+// The steps are cut into segments, one per CTA, and a segment into runs of kRun steps, one
+// per thread. A run takes the advantage x after it to b + p x before it, with p the product
+// of its decays; such maps compose, so a thread forms its run's map from its own steps, the
+// CTA composes the runs', and the first kernel leaves the segment's map. The second kernel
+// composes the maps of the segments after its own, which is the advantage that follows it,
+// and walks its runs again with that.
+constexpr int kRun = 8;
+constexpr int kCtaThreads = 256;
+
+template <typename T> struct Map {
+  T p, b;  // x -> b + p x
+};
+// an end of an episode (p = 0) keeps whatever is after it out, NaN included
+template <typename T> __device__ __forceinline__ Map<T> after(Map<T> first, Map<T> then) {
+  // `first` is the earlier stretch of time: x -> first(then(x))
+  return Map<T>{first.p * then.p, first.p == T(0) ? first.b : first.b + first.p * then.b};
+}
+template <typename T> __device__ __forceinline__ T apply(Map<T> m, T x) {
+  return m.p == T(0) ? m.b : m.b + m.p * x;
+}
+
+// Columns per CTA: a power of two up to 32, the least that holds them all.
+inline int tile_columns(long long columns) {
+  int c = 1;
+  while (c < 32 && c < columns) c *= 2;
+  return c;
+}
+
+template <typename T, bool FINAL>
+__global__ void __launch_bounds__(kCtaThreads)
+    gae_segments_kernel(Args<T> a, int tile, long long segments, Map<T>* maps) {
+  __shared__ Map<T> runs[kCtaThreads];
+  const int c = threadIdx.x % tile, q = threadIdx.x / tile, n = kCtaThreads / tile;
+  const long long seg = blockIdx.x, j = blockIdx.y * static_cast<long long>(tile) + c;
+  const bool in = j < a.columns;
+  const long long f = in ? j / a.per_flag : 0;
+  const long long t0 = (seg * n + q) * kRun;  // the run's first step
+  Step<T> s[kRun];
+  T after_v = 0;
+#pragma unroll
+  for (int k = 0; k < kRun; ++k)
+    if (in && t0 + k < a.steps) s[k] = load_step(a, t0 + k, j, f);
+  if (in && !a.next && t0 < a.steps)
+    after_v = t0 + kRun < a.steps ? a.v[(t0 + kRun) * a.columns + j] : a.last[j];
+  T x = 0;  // the advantage after the CTA's segment
+  if (FINAL) {
+    // the later segments in n parts, then the parts in order
+    const long long later = segments - 1 - seg, each = (later + n - 1) / n;
+    Map<T> m{T(1), T(0)};
+    for (long long k = seg + 1 + q * each; in && k < seg + 1 + min((q + 1) * each, later); ++k)
+      m = after(m, maps[k * a.columns + j]);
+    runs[threadIdx.x] = m;
+    __syncthreads();
+    for (int k = n - 1; k >= 0; --k) x = apply(runs[k * tile + c], x);
+    __syncthreads();
+  }
+  T d[kRun];
+  Map<T> m{T(1), T(0)};
+#pragma unroll
+  for (int k = kRun - 1; k >= 0; --k) {
+    d[k] = 0;
+    if (in && t0 + k < a.steps) {
+      d[k] = s[k].r + (s[k].term ? T(0) : a.gamma * (a.next ? s[k].next : after_v)) - s[k].v;
+      after_v = s[k].v;
+      m = after(Map<T>{s[k].stop ? T(0) : a.decay, d[k]}, m);
+    }
+  }
+  runs[threadIdx.x] = m;
+  __syncthreads();
+  if constexpr (FINAL) {
+    for (int k = n - 1; k > q; --k) x = apply(runs[k * tile + c], x);
+#pragma unroll
+    for (int k = kRun - 1; k >= 0; --k) {
+      if (in && t0 + k < a.steps) {
+        x = s[k].stop ? d[k] : d[k] + a.decay * x;
+        const long long at = (t0 + k) * a.columns + j;
+        a.adv[at] = x;
+        a.ret[at] = x + s[k].v;
+      }
+    }
+  } else if (q == 0 && in) {
+    for (int k = 1; k < n; ++k) m = after(m, runs[k * tile + c]);
+    maps[seg * a.columns + j] = m;
+  }
+}
+
+// Threads of their own for all columns keep the memory busy from about this many on.
+constexpr long long kManyColumns = 32768;
+
+struct Plan {
+  bool split;
+  int tile;
+  long long segments;
+  size_t bytes;
+};
+Plan plan_of(const swarp_gae_t* g) {
+  Plan q{};
+  q.tile = tile_columns(g->columns);
+  q.split = g->columns < kManyColumns && g->steps > kRun;
+  if (q.split) {
+    const long long per = static_cast<long long>(kCtaThreads / q.tile) * kRun;
+    q.segments = (g->steps + per - 1) / per;
+    const size_t one = g->dtype == SWARP_F32 ? sizeof(Map<float>) : sizeof(Map<double>);
+    if (q.segments > 1) q.bytes = one * q.segments * g->columns;
+  }
+  return q;
 }
 
 int check(const swarp_gae_t* g) {
@@ -42,12 +176,23 @@ int check(const swarp_gae_t* g) {
   return SWARP_OK;
 }
 
-template <typename T> int run(const swarp_gae_t* g, cudaStream_t st) {
+template <typename T> int run(const swarp_gae_t* g, const Plan& q, void* ws, cudaStream_t st) {
   Args<T> a{static_cast<const T*>(g->rewards), static_cast<const T*>(g->values),
             static_cast<const T*>(g->next_values), static_cast<const T*>(g->last_values),
             g->terminated, g->truncated, static_cast<T*>(g->advantages),
             static_cast<T*>(g->returns), g->steps, g->columns, g->columns / g->columns_per_flag,
             g->columns_per_flag, static_cast<T>(g->gamma), static_cast<T>(g->gamma * g->lambda)};
+  if (q.split) {
+    Map<T>* maps = static_cast<Map<T>*>(ws);
+    const long long tiles = (g->columns + q.tile - 1) / q.tile;
+    const dim3 grid(static_cast<unsigned>(q.segments), static_cast<unsigned>(tiles));
+    if (q.segments > 1) {
+      gae_segments_kernel<T, false><<<grid, kCtaThreads, 0, st>>>(a, q.tile, q.segments, maps);
+      if (const int rc = launch_status()) return rc;
+    }
+    gae_segments_kernel<T, true><<<grid, kCtaThreads, 0, st>>>(a, q.tile, q.segments, maps);
+    return launch_status();
+  }
   gae_columns_kernel<T><<<(unsigned)((g->columns + 255) / 256), 256, 0, st>>>(a);
   return launch_status();
 }
@@ -61,8 +206,7 @@ using namespace swarp::learn;
 extern "C" {
 
 size_t swarp_gae_workspace_bytes(const swarp_gae_t* g) {
-  (void)g;
-  return 0;
+  return check(g) == SWARP_OK ? plan_of(g).bytes : 0;
 }
 
 int swarp_gae(const swarp_gae_t* g, void* workspace, size_t workspace_bytes, void* stream) {
@@ -71,10 +215,11 @@ int swarp_gae(const swarp_gae_t* g, void* workspace, size_t workspace_bytes, voi
   if (!g->rewards || !g->values || !g->advantages || !g->returns ||
       (!g->next_values && !g->last_values))
     return SWARP_ERR_INVALID_ARG;
-  const size_t need = swarp_gae_workspace_bytes(g);
-  if (need > 0 && (!workspace || workspace_bytes < need)) return SWARP_ERR_WORKSPACE;
+  const Plan q = plan_of(g);
+  if (q.bytes > 0 && (!workspace || workspace_bytes < q.bytes)) return SWARP_ERR_WORKSPACE;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return g->dtype == SWARP_F32 ? run<float>(g, st) : run<double>(g, st);
+  return g->dtype == SWARP_F32 ? run<float>(g, q, workspace, st)
+                               : run<double>(g, q, workspace, st);
 }
 
 }  // extern "C"
