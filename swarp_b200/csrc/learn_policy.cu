@@ -6,6 +6,9 @@
 //   dloss/dlp = c = -r A where the clip does not cut, + kl (1 - e^(ref - lp))
 //   dloss/dz_j = c (1{j = a} - p_j) + ent p_j (ln p_j + H),        p_j = e^(z_j - m) / S
 // so one row needs its maximum, two sums, and then one more look at its logits.
+#include <atomic>
+#include <type_traits>
+
 #include "learn.cuh"
 
 namespace swarp {
@@ -58,23 +61,38 @@ struct Row {
   float c;  // d(row loss) / d(lp)
 };
 
-// The scalar part of a row from its log probability and entropy.
-__device__ __forceinline__ Row row_terms(const Args& a, long long i, float lp, float H,
+// What a row's scalar part reads; the kernels load it ahead of the row.
+struct Inputs {
+  float old, adv, ref;
+};
+__device__ __forceinline__ Inputs inputs_of(const Args& a, long long i) {
+  Inputs x{0.f, 0.f, 0.f};
+  if (a.with_loss) {
+    x.old = a.old_logp[i];
+    x.adv = a.advantages[i];
+    if (a.ref_logp) x.ref = a.ref_logp[i];
+  }
+  return x;
+}
+
+// The scalar part of a row from its log probability and entropy. The exponentials are good to
+// a few ulp at the arguments that a ratio or a divergence has.
+__device__ __forceinline__ Row row_terms(const Args& a, const Inputs& x, float lp, float H,
                                          bool empty) {
   Row r{lp, H, 0.f, 0.f, 0.f, 0.f};
   if (empty || !a.with_loss) return r;
-  const float A = a.advantages[i];
-  const float ratio = expf(lp - a.old_logp[i]);
+  const float A = x.adv;
+  const float ratio = exp2_fast((lp - x.old) * kLog2e);
   const float bounded = fminf(fmaxf(ratio, 1.f - a.lo), 1.f + a.hi);
-  const float s1 = ratio * A, s2 = (ratio != ratio ? ratio : bounded) * A;
+  const float s1 = ratio * A, s2 = bounded * A;
   r.pg = s1 != s1 ? -s1 : -fminf(s1, s2);
   const bool cut = (A > 0.f && ratio > 1.f + a.hi) || (A < 0.f && ratio < 1.f - a.lo);
   r.cut = cut ? 1.f : 0.f;
   r.c = cut ? 0.f : -s1;
   if (a.ref_logp) {
-    const float d = a.ref_logp[i] - lp;
-    r.k3 = expm1f(d) - d;
-    if (a.kl != 0.f) r.c -= a.kl * expm1f(d);
+    const float d = x.ref - lp, e1 = exp2_fast(d * kLog2e) - 1.f;
+    r.k3 = e1 - d;
+    if (a.kl != 0.f) r.c -= a.kl * e1;
   }
   return r;
 }
@@ -146,15 +164,20 @@ __global__ void __launch_bounds__(kGroupThreads) policy_group_kernel(Args a) {
     const unsigned lives = __ballot_sync(kAll, live) >> base;
     long long tok = -1;
     float za = 0.f;
+    Inputs in0{0.f, 0.f, 0.f};
     if (live) {
+      in0 = inputs_of(a, i);
       tok = token_of(a, i);
       za = NAN;
       if (tok >= 0 && tok < V) za = to_f((static_cast<const T*>(a.logits) + row_offset(a, i))[tok]);
     }
     float z[R][E];
+    const bool flat = a.inner == a.rows;
+    const T* p0 = static_cast<const T*>(a.logits) + i0 * a.stride_inner;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const T* p = static_cast<const T*>(a.logits) + row_offset(a, i0 + r);
+      const T* p = flat ? p0 + r * a.stride_inner
+                        : static_cast<const T*>(a.logits) + row_offset(a, i0 + r);
       const bool in = lives >> (r * kPerRow) & 1u;
 #pragma unroll
       for (int k = 0; k < E; ++k) {
@@ -187,8 +210,8 @@ __global__ void __launch_bounds__(kGroupThreads) policy_group_kernel(Args a) {
       }
     }
     const float s = reduce_rows<L, R>(v, l, plus), t = reduce_rows<L, R>(u, l, plus);
-    const float ln = empty ? 0.f : logf(s), inv = empty ? 0.f : 1.f / s;
-    const Row row = row_terms(a, i, empty ? (za != za ? za : -INFINITY) : (za - m) - ln,
+    const float ln = empty ? 0.f : __logf(s), inv = empty ? 0.f : __fdividef(1.f, s);
+    const Row row = row_terms(a, in0, empty ? (za != za ? za : -INFINITY) : (za - m) - ln,
                               ln - t * inv, !live || (empty && za == za));
     if (l % kPerRow == 0 && live) {
       sums[0] += row.pg, sums[1] += row.k3, sums[2] += row.H, sums[3] += row.cut;
@@ -232,6 +255,121 @@ __global__ void __launch_bounds__(kGroupThreads) policy_group_kernel(Args a) {
       for (int q = 0; q < kGroupThreads / 32; ++q) x += part[q][threadIdx.x];
       a.partials[blockIdx.x * 4ll + threadIdx.x] = x * w;
     }
+  }
+}
+
+// Many short rows that lie one after the other: a CTA brings 128 of them into shared memory in
+// whole vectors, a thread takes one row from there, and the gradients go back the same way.
+// No lane waits for another's sums, and nothing is computed twice.
+constexpr int kTileRows = 128;
+
+template <typename T, int E, bool GRAD>
+__global__ void __launch_bounds__(kTileRows) policy_tile_kernel(Args a) {
+  constexpr int N = 16 / sizeof(T), kCopies = kTileRows * E / N / kTileRows;
+  __shared__ __align__(16) T tile[kTileRows * E];
+  __shared__ double part[kTileRows / 32][4];
+  const float cot = a.cotangent ? *a.cotangent : 1.f;
+  if (a.skip_unit && cot == 1.f) return;
+  const float w = row_weight(a), wg = w * a.grad_scale * cot;
+  const int V = static_cast<int>(a.vocab), tid = threadIdx.x;
+  // A row starts tid V elements in. Where that would put many threads on one bank they start
+  // at different places of their rows.
+  const int turn = sizeof(T) == 4 ? (V % 2 == 0 ? tid % V : 0) : (V % 4 == 0 ? 2 * tid % V : 0);
+  auto place = [&](int k) {
+    const int j = k + turn;
+    return tid * V + (j >= V ? j - V : j);
+  };
+  double sums[4] = {0, 0, 0, 0};
+  for (long long base = static_cast<long long>(blockIdx.x) * kTileRows; base < a.rows;
+       base += static_cast<long long>(gridDim.x) * kTileRows) {
+    const int n = static_cast<int>(min(a.rows - base, static_cast<long long>(kTileRows)));
+    const int cells = n * V, vecs = cells / N;
+    const long long i = base + tid;
+    {
+      const T* z = static_cast<const T*>(a.logits) + base * V;
+      uint4 q[kCopies];
+#pragma unroll
+      for (int k = 0; k < kCopies; ++k)
+        if (k * kTileRows + tid < vecs)
+          q[k] = *(reinterpret_cast<const uint4*>(z) + k * kTileRows + tid);
+      if (vecs * N + tid < cells) tile[vecs * N + tid] = z[vecs * N + tid];
+#pragma unroll
+      for (int k = 0; k < kCopies; ++k)
+        if (k * kTileRows + tid < vecs) reinterpret_cast<uint4*>(tile)[k * kTileRows + tid] = q[k];
+    }
+    const bool in = tid < n, live = in && (!a.mask || a.mask[i]);
+    const long long tok = live ? token_of(a, i) : 0;
+    const Inputs in0 = live ? inputs_of(a, i) : Inputs{0.f, 0.f, 0.f};
+    __syncthreads();
+    if (live) {
+      float z[E];
+      float m = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < E; ++k)
+        if (k < V) m = max_nan(m, z[k] = to_f(tile[place(k)]));
+      const float za = tok >= 0 && tok < V ? to_f(tile[tid * V + static_cast<int>(tok)]) : NAN;
+      const bool empty = m == -INFINITY;
+      if (empty) m = 0.f;
+      float s = 0.f, t = 0.f;
+#pragma unroll
+      for (int k = 0; k < E; ++k)
+        if (k < V) {
+          const float x = max_nan(z[k] - m, -1e4f);  // so that 0 x stays 0
+          z[k] = exp2_fast(x * kLog2e);
+          s += z[k];
+          t = fmaf(z[k], x, t);
+        }
+      const float ln = empty ? 0.f : __logf(s), inv = empty ? 0.f : __fdividef(1.f, s);
+      const Row r = row_terms(a, in0, empty ? (za != za ? za : -INFINITY) : (za - m) - ln,
+                              ln - t * inv, empty && za == za);
+      sums[0] += r.pg, sums[1] += r.k3, sums[2] += r.H, sums[3] += r.cut;
+      if (a.logp) a.logp[i] = r.lp, a.entropy[i] = r.H;
+      if (GRAD) {
+        const float c = wg * r.c, eta = wg * a.ent;
+        const float k0 = inv * (eta * (r.H - ln) - c), k1 = inv * eta;
+        const bool with_ent = a.ent != 0.f;
+#pragma unroll
+        for (int k = 0; k < E; ++k)
+          if (k < V) {
+            T& at = tile[place(k)];
+            float f = k0;
+            if (with_ent) f = fmaf(k1, max_nan(to_f(at) - m, -1e4f), k0);
+            at = from_f<T>(z[k] * f);
+          }
+        if (tok >= 0 && tok < V) {
+          const float x = max_nan(za - m, -1e4f);
+          tile[tid * V + static_cast<int>(tok)] =
+              from_f<T>(exp2_fast(x * kLog2e) * fmaf(k1, x, k0) + c);
+        }
+      }
+    } else if (in) {
+      if (a.logp) a.logp[i] = 0.f, a.entropy[i] = 0.f;
+      if (GRAD)
+        for (int k = 0; k < V; ++k) tile[tid * V + k] = from_f<T>(0.f);
+    }
+    __syncthreads();
+    if (GRAD) {
+      T* g = static_cast<T*>(a.grad) + base * V;
+#pragma unroll
+      for (int k = 0; k < kCopies; ++k)
+        if (k * kTileRows + tid < vecs)
+          reinterpret_cast<uint4*>(g)[k * kTileRows + tid] =
+              reinterpret_cast<const uint4*>(tile)[k * kTileRows + tid];
+      if (vecs * N + tid < cells) g[vecs * N + tid] = tile[vecs * N + tid];
+      __syncthreads();
+    }
+  }
+  if (!a.partials) return;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    sums[k] = warp_sum(sums[k]);
+    if ((tid & 31) == 0) part[tid >> 5][k] = sums[k];
+  }
+  __syncthreads();
+  if (tid < 4) {
+    double x = 0;
+    for (int q = 0; q < kTileRows / 32; ++q) x += part[q][tid];
+    a.partials[blockIdx.x * 4ll + tid] = x * w;
   }
 }
 
@@ -309,32 +447,6 @@ template <> struct Vec<__half> {
   }
 };
 
-// two floats as one operand of the packed instructions
-struct F2 {
-  unsigned long long v;
-  __device__ __forceinline__ F2(float2 f) {
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(f.x), "f"(f.y));
-  }
-  __device__ __forceinline__ F2(float x) : F2(make_float2(x, x)) {}
-  __device__ __forceinline__ float2 f() const {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-  }
-};
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
-  return a;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
-  return a;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c.v) : "l"(a.v), "l"(b.v));
-  return c;
-}
-
 // A part of a row: the maximum of its logits, and its sums of e^x and e^x x with x counted
 // from that maximum (from 0 where all are -inf).
 struct Part {
@@ -364,186 +476,296 @@ __device__ __forceinline__ uint4 load_once(const uint4* p) {
   return q;
 }
 
-__device__ __forceinline__ void cluster_arrive() {
+__device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t shared_at(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void mbar_init(uint64_t* b) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_at(b)) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint64_t* b, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_at(b)),
+               "r"(bytes)
+               : "memory");
+}
+// whether the phase came to its end before the limit (about a second)
+__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity) {
+  const uint32_t at = shared_at(b);
+  for (int k = 0; k < (1 << 20); ++k) {
+    uint32_t done;
+    asm volatile(
+        "{ .reg .pred p;\n"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p; }"
+        : "=r"(done)
+        : "r"(at), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+// p to the same place in the shared memory of CTA `to` of the cluster, counted by its barrier
+__device__ __forceinline__ void send(float4* place, uint64_t* bar, int to, Part p) {
+  uint32_t d, b;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(shared_at(place)), "r"(to));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(shared_at(bar)), "r"(to));
+  asm volatile(
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, "
+      "%4}, [%5];" ::"r"(d),
+      "f"(p.m), "f"(p.s), "f"(p.t), "f"(0.f), "r"(b)
+      : "memory");
+}
+
+// A row as a thread of its group sees it: whole vectors, and up to N - 1 elements before and
+// after them with one thread each.
+template <typename T> struct Cut {
+  const uint4* vec;
+  int vecs, head, edge;
+  __device__ __forceinline__ Cut(const T* z, int V, int at) {
+    head = min(V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) /
+                      static_cast<int>(sizeof(T)));
+    vecs = (V - head) / Vec<T>::N;
+    vec = reinterpret_cast<const uint4*>(z + head);
+    const int tail = head + vecs * Vec<T>::N;
+    edge = at < head ? at : at >= 16 && at - 16 < V - tail ? tail + at - 16 : -1;
+  }
+};
+
+constexpr int split_block(int threads) { return threads == 32 ? 256 : threads; }
+// CTAs per SM that the registers have to allow: 24 warps of 80 registers, 16 of 128
+constexpr int split_resident(int threads, int nv) {
+  return (nv > 8 ? 512 : 768) / split_block(threads);
 }
 
 // THREADS = 32: one row per warp, 8 warps per CTA, C = 1. Otherwise one row per cluster of C
-// CTAs of THREADS.
+// CTAs of THREADS. The CTAs are resident ones that walk the rows. With a gradient, a vector's
+// registers take the next row's vector as soon as its gradient is out, so the next row is on
+// its way while this one is written. The parts of a row go to all CTAs of the cluster by
+// asynchronous stores that a barrier in the receiver's shared memory counts: a cluster
+// barrier would first wait for the gradient's stores.
 template <typename T, int NV, int THREADS, int C, bool GRAD>
-__global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) policy_split_kernel(Args a) {
+__global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS, NV))
+    policy_split_kernel(Args a) {
   constexpr bool kWarp = THREADS == 32;
   constexpr int kWarps = kWarp ? 1 : THREADS / 32;
   constexpr int N = Vec<T>::N;
   constexpr int kAllThreads = THREADS * C;
-  __shared__ float4 parts[2][kWarp ? 1 : C * kWarps];
+  constexpr int kParts = C * kWarps;
+  __shared__ float4 parts[2][kWarp ? 1 : kParts];
+  __shared__ uint64_t bars[2];
   const float cot = a.cotangent ? *a.cotangent : 1.f;
   if (a.skip_unit && cot == 1.f) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = C > 1 ? static_cast<int>(blockIdx.x % C) : 0;  // clusters are runs of C CTAs
   const int at = kWarp ? lane : rank * THREADS + static_cast<int>(threadIdx.x);
-  if (C > 1) cluster_arrive(), cluster_wait();  // every CTA's shared memory is there
+  // the warp's first place, known to be the same in all its lanes
+  const int warp_at = __shfl_sync(kAll, at, 0);
+  if (C > 1) {
+    if (threadIdx.x == 0) {
+      mbar_init(&bars[0]), mbar_init(&bars[1]);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    cluster_sync();
+  }
   const float w = row_weight(a), wg = w * a.grad_scale * cot;
   const long long first = kWarp ? blockIdx.x * 8ll + warp : blockIdx.x / C;
   const long long step = kWarp ? gridDim.x * 8ll : gridDim.x / C;
+  const int V = static_cast<int>(a.vocab);
   double sums[4] = {0, 0, 0, 0};
   int turn = 0;
-  for (long long i = first; i < a.rows; i += step) {
-    T* g = GRAD ? static_cast<T*>(a.grad) + i * a.vocab : nullptr;
-    const int V = static_cast<int>(a.vocab);
-    if (a.mask && !a.mask[i]) {  // the same for all threads of the row
+  bool lost = false;  // a part did not come: all that follows is NaN
+
+  // the first row from i on that the mask admits; those before it get their zeros
+  auto admitted = [&](long long i) {
+    for (; i < a.rows && a.mask && !a.mask[i]; i += step) {
       if (GRAD) {
-        const int head = min(V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(g) & 15)) & 15) /
-                                    static_cast<int>(sizeof(T)));
-        const int vecs = (V - head) / N;
-        uint4* q = reinterpret_cast<uint4*>(g + head);
-        for (int k = at; k < vecs; k += kAllThreads) q[k] = make_uint4(0, 0, 0, 0);
-        if (at < head) g[at] = from_f<T>(0.f);
-        const int tail = head + vecs * N;
-        if (at < V - tail) g[tail + at] = from_f<T>(0.f);
+        T* g = static_cast<T*>(a.grad) + i * V;
+        const Cut<T> cut(g, V, at);
+        uint4* gv = reinterpret_cast<uint4*>(g + cut.head);
+        for (int k = at; k < cut.vecs; k += kAllThreads) gv[k] = make_uint4(0, 0, 0, 0);
+        if (cut.edge >= 0) g[cut.edge] = from_f<T>(0.f);
       }
       if (at == 0 && a.logp) a.logp[i] = 0.f, a.entropy[i] = 0.f;
-      continue;
     }
-    const T* z = static_cast<const T*>(a.logits) + row_offset(a, i);
-    const long long tok = token_of(a, i);
-    // whole vectors, and up to N - 1 elements before and after them with one thread each
-    const int head = min(V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) /
-                                static_cast<int>(sizeof(T)));
-    const int vecs = (V - head) / N, tail = head + vecs * N;
-    const uint4* zv = reinterpret_cast<const uint4*>(z + head);
-    uint4 q[NV];
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int j = k * kAllThreads + at;
-      q[k] = make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
-      if (j < vecs) q[k] = load_once(zv + j);
-    }
-    const int edge = at < head ? at : at >= 16 && at - 16 < V - tail ? tail + at - 16 : -1;
-    const float ze = edge >= 0 ? to_f(z[edge]) : -INFINITY;
-    const float za = tok >= 0 && tok < V ? to_f(z[tok]) : NAN;
+    return i;
+  };
+  auto start_of = [&](long long i) { return static_cast<const T*>(a.logits) + row_offset(a, i); };
+  auto at_token = [&](const T* z, long long tok) {
+    return tok >= 0 && tok < V ? to_f(z[tok]) : NAN;
+  };
+  // vector k of the row that `cut` describes; -inf in the lanes beyond its end
+  auto fetch = [&](const Cut<T>& cut, int k) {
+    const int j = k * kAllThreads + at;
+    uint4 q = make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
+    if (j < cut.vecs) q = load_once(cut.vec + j);
+    return q;
+  };
 
-    Part p{ze, 0.f, 0.f};
+  long long i = admitted(first);
+  if (i < a.rows) {
+    uint4 q[NV];
+    const T* z = start_of(i);
+    Cut<T> cut(z, V, at);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) p.m = Vec<T>::most(q[k], p.m);
-    {
-      const F2 o(-origin(p.m)), scale(kLog2e);
-      F2 s(0.f), t(0.f);
+    for (int k = 0; k < NV; ++k) q[k] = fetch(cut, k);
+    float ze = cut.edge >= 0 ? to_f(z[cut.edge]) : -INFINITY;
+    long long tok = token_of(a, i);
+    Inputs in = inputs_of(a, i);
+    float za = at_token(z, tok);
+    bool low = false;  // the thread has met a logit of -inf: its products need care
+    while (true) {
+      Part p{ze, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
+      for (int k = 0; k < NV; ++k)
+        if (k * kAllThreads + warp_at < cut.vecs) p.m = Vec<T>::most(q[k], p.m);
+      {
+        const float o = origin(p.m);
+        auto sum = [&](auto bounded) {
+          float s[2] = {0.f, 0.f}, t[2] = {0.f, 0.f};
 #pragma unroll
-        for (int h = 0; h < N / 2; ++h) {
-          float2 x = add2(F2(Vec<T>::pair(q[k], h)), o).f();
-          x.x = max_nan(x.x, -1e4f), x.y = max_nan(x.y, -1e4f);  // so that 0 x stays 0
-          float2 e = mul2(F2(x), scale).f();
-          e.x = exp2_fast(e.x), e.y = exp2_fast(e.y);
-          s = add2(s, F2(e));
-          t = fma2(F2(e), F2(x), t);
-        }
+          for (int k = 0; k < NV; ++k)
+            if (k * kAllThreads + warp_at < cut.vecs) {
+#pragma unroll
+              for (int h = 0; h < N / 2; ++h) {
+                float2 x = Vec<T>::pair(q[k], h);
+                x.x -= o, x.y -= o;
+                if (decltype(bounded)::value) x.x = max_nan(x.x, -1e4f), x.y = max_nan(x.y, -1e4f);
+                const float e0 = exp2_fast(x.x * kLog2e), e1 = exp2_fast(x.y * kLog2e);
+                s[0] += e0, s[1] += e1;
+                t[0] = fmaf(e0, x.x, t[0]), t[1] = fmaf(e1, x.y, t[1]);
+              }
+            }
+          const float x = max_nan(ze - o, -1e4f), e = exp2_fast(x * kLog2e);
+          p.s = s[0] + s[1] + e;
+          p.t = fmaf(e, x, t[0] + t[1]);
+        };
+        if (!low) sum(std::false_type{});
+        // 0 times -inf: again with x bounded below, and so from now on
+        if (low || p.t != p.t) low = true, sum(std::true_type{});
       }
-      const float x = max_nan(ze - origin(p.m), -1e4f), e = exp2_fast(x * kLog2e);
-      p.s = s.f().x + s.f().y + e;
-      p.t = fmaf(e, x, t.f().x + t.f().y);
-    }
-    p = warp_join(p);
-    if (!kWarp) {
-      if (C == 1) {
-        if (lane == 0) parts[turn][warp] = make_float4(p.m, p.s, p.t, 0.f);
-        __syncthreads();
-      } else {
-        // every warp's part goes to all CTAs of the cluster
-        if (lane < C) {
-          uint32_t to, from = static_cast<uint32_t>(
-                           __cvta_generic_to_shared(&parts[turn][rank * kWarps + warp]));
-          asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(from), "r"(lane));
-          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(p.m),
-                       "f"(p.s), "f"(p.t), "f"(0.f)
-                       : "memory");
-        }
-        cluster_arrive();
-        cluster_wait();
+      // the next row, and what can be asked of it already
+      const long long i2 = admitted(i + step);
+      const bool more = i2 < a.rows;
+      const T* z2 = more ? start_of(i2) : z;
+      const Cut<T> cut2(z2, more ? V : 0, at);
+      const long long tok2 = more ? token_of(a, i2) : -1;
+      const Inputs in2 = more ? inputs_of(a, i2) : in;
+      if (!GRAD) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) q[k] = fetch(cut2, k);
       }
-      constexpr int kParts = C * kWarps, kEach = (kParts + 31) / 32;
-      Part mine[kEach];
-      float top = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < kEach; ++k) {
-        const int j = lane + 32 * k;
-        mine[k] = Part{-INFINITY, 0.f, 0.f};
-        if (j < kParts) {
-          const float4 f = parts[turn][j];
-          mine[k] = Part{f.x, f.y, f.z};
-        }
-        top = max_nan(top, mine[k].m);
-      }
-      top = warp_max(top);
-      p = Part{top, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < kEach; ++k) {
-        onto(mine[k], top);
-        p.s += mine[k].s;
-        p.t += mine[k].t;
-      }
-      p.s = warp_sum(p.s);
-      p.t = warp_sum(p.t);
-      // the next row's parts go to the other buffer; the one after that comes past another
-      // barrier, which nobody passes before all have read these
-      turn ^= 1;
-    }
-    const bool empty = p.m == -INFINITY;
-    const float m = origin(p.m), ln = empty ? 0.f : logf(p.s), inv = empty ? 0.f : 1.f / p.s;
-    const Row r = row_terms(a, i, empty ? (za != za ? za : -INFINITY) : (za - m) - ln,
-                            ln - p.t * inv, empty && za == za);
-    if (at == 0) {
-      if (a.logp) a.logp[i] = r.lp, a.entropy[i] = r.H;
-      sums[0] += r.pg, sums[1] += r.k3, sums[2] += r.H, sums[3] += r.cut;
-    }
-    if (GRAD) {
-      const float c = wg * r.c, eta = wg * a.ent;
-      const float k0 = inv * (eta * (r.H - ln) - c), k1 = inv * eta;
-      uint4* gv = reinterpret_cast<uint4*>(g + head);
-      const bool same_phase = ((reinterpret_cast<uintptr_t>(gv)) & 15) == 0;
-      const F2 o(-m), scale(kLog2e), f0(k0), f1(k1);
-      // the vector and the place in it of the token, if this thread holds it
-      const int tk = tok >= 0 && tok < V ? static_cast<int>(tok) : -1, tv = tk - head;
-      const int tvec = tv >= 0 && tv < vecs * N ? tv / N : -1;
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int j = k * kAllThreads + at;
-        if (j >= vecs) break;
-        uint4 out;
-#pragma unroll
-        for (int h = 0; h < N / 2; ++h) {
-          float2 x = add2(F2(Vec<T>::pair(q[k], h)), o).f();
-          if (a.ent != 0.f) x.x = max_nan(x.x, -1e4f), x.y = max_nan(x.y, -1e4f);
-          float2 e = mul2(F2(x), scale).f();
-          e.x = exp2_fast(e.x), e.y = exp2_fast(e.y);
-          float2 d = mul2(F2(e), a.ent != 0.f ? fma2(f1, F2(x), f0) : f0).f();
-          if (j == tvec) {
-            if (tv % N == 2 * h) d.x += c;
-            if (tv % N == 2 * h + 1) d.y += c;
-          }
-          Vec<T>::set(out, h, d);
-        }
-        if (same_phase) {
-          gv[j] = out;
+      p = warp_join(p);
+      if (!kWarp) {
+        float4* box = parts[turn & 1];
+        if (C == 1) {
+          if (lane == 0) box[warp] = make_float4(p.m, p.s, p.t, 0.f);
+          __syncthreads();
         } else {
-          const T* o8 = reinterpret_cast<const T*>(&out);
+          uint64_t* bar = &bars[turn & 1];
+          if (threadIdx.x == 0) mbar_expect(bar, kParts * sizeof(float4));
+          if (lane < C) send(&box[rank * kWarps + warp], bar, lane, p);
+          if (!lost) lost = !mbar_wait(bar, (turn >> 1) & 1);
+        }
+        constexpr int kEach = (kParts + 31) / 32;
+        Part mine[kEach];
+        float top = lost ? NAN : -INFINITY;
 #pragma unroll
-          for (int h = 0; h < N; ++h) g[head + j * N + h] = o8[h];
+        for (int k = 0; k < kEach; ++k) {
+          const int j = lane + 32 * k;
+          mine[k] = Part{-INFINITY, 0.f, 0.f};
+          if (j < kParts) {
+            const float4 f = box[j];
+            mine[k] = Part{f.x, f.y, f.z};
+          }
+          top = max_nan(top, mine[k].m);
+        }
+        top = warp_max(top);
+        p = Part{top, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+          onto(mine[k], top);
+          p.s += mine[k].s;
+          p.t += mine[k].t;
+        }
+        p.s = warp_sum(p.s);
+        p.t = warp_sum(p.t);
+        // The next row's parts go to the other box. The one after that comes to this box only
+        // when its sender holds all of the next row's parts, and every warp sends its own of
+        // those after it has read this box.
+        ++turn;
+      }
+      const bool empty = p.m == -INFINITY;
+      const float m = origin(p.m);
+      const float ln = empty ? 0.f : __logf(p.s), inv = empty ? 0.f : __fdividef(1.f, p.s);
+      const Row r = row_terms(a, in, empty ? (za != za ? za : -INFINITY) : (za - m) - ln,
+                              ln - p.t * inv, empty && za == za);
+      if (at == 0) {
+        if (a.logp) a.logp[i] = r.lp, a.entropy[i] = r.H;
+        sums[0] += r.pg, sums[1] += r.k3, sums[2] += r.H, sums[3] += r.cut;
+      }
+      if (GRAD) {
+        const float c = wg * r.c, eta = wg * a.ent;
+        const float k0 = inv * (eta * (r.H - ln) - c), k1 = inv * eta;
+        T* g = static_cast<T*>(a.grad) + i * V;
+        uint4* gv = reinterpret_cast<uint4*>(g + cut.head);
+        const bool same_phase = (reinterpret_cast<uintptr_t>(gv) & 15) == 0;
+        // kind 0: no entropy term; 1: with it; 2: with it, x bounded
+        auto write = [&](auto kind) {
+          constexpr int kKind = decltype(kind)::value;
+#pragma unroll
+          for (int k = 0; k < NV; ++k) {
+            if (k * kAllThreads + warp_at < cut.vecs) {
+              const int j = k * kAllThreads + at;
+              uint4 out;
+#pragma unroll
+              for (int h = 0; h < N / 2; ++h) {
+                float2 x = Vec<T>::pair(q[k], h);
+                x.x -= m, x.y -= m;
+                if (kKind == 2) x.x = max_nan(x.x, -1e4f), x.y = max_nan(x.y, -1e4f);
+                const float e0 = exp2_fast(x.x * kLog2e), e1 = exp2_fast(x.y * kLog2e);
+                Vec<T>::set(out, h, kKind == 0 ? make_float2(e0 * k0, e1 * k0)
+                                               : make_float2(e0 * fmaf(k1, x.x, k0),
+                                                             e1 * fmaf(k1, x.y, k0)));
+              }
+              if (j < cut.vecs) {
+                if (same_phase) {
+                  gv[j] = out;
+                } else {
+                  const T* o8 = reinterpret_cast<const T*>(&out);
+#pragma unroll
+                  for (int h = 0; h < N; ++h) g[cut.head + j * N + h] = o8[h];
+                }
+              }
+            }
+            q[k] = fetch(cut2, k);
+          }
+        };
+        if (a.ent == 0.f) write(std::integral_constant<int, 0>{});
+        else if (!low) write(std::integral_constant<int, 1>{});
+        else write(std::integral_constant<int, 2>{});
+        auto alone = [&](float zj) {
+          const float x = max_nan(zj - m, -1e4f);
+          return exp2_fast(x * kLog2e) * fmaf(k1, x, k0);
+        };
+        if (cut.edge >= 0) g[cut.edge] = from_f<T>(alone(ze));
+        // the token's own place again, by the thread that has just written it
+        if (tok >= 0 && tok < V) {
+          const int j = static_cast<int>(tok) - cut.head;
+          const bool mine = j >= 0 && j < cut.vecs * N ? j / N % kAllThreads == at
+                                                       : cut.edge == static_cast<int>(tok);
+          if (mine) g[tok] = from_f<T>(alone(za) + c);
         }
       }
-      if (edge >= 0) {
-        const float x = max_nan(ze - m, -1e4f);
-        float d = exp2_fast(x * kLog2e) * fmaf(k1, x, k0);
-        if (edge == tk) d += c;
-        g[edge] = from_f<T>(d);
-      }
+      if (!more) break;
+      i = i2, z = z2, cut = cut2, tok = tok2, in = in2;
+      ze = cut.edge >= 0 ? to_f(z[cut.edge]) : -INFINITY;
+      za = at_token(z, tok);
     }
   }
+  if (C > 1) cluster_sync();  // nobody leaves while a part may still be on its way to it
   if (!a.partials) return;
   if (kWarp) {
     __shared__ double part[8][4];
@@ -618,7 +840,8 @@ __global__ void __launch_bounds__(kLoopThreads) policy_loop_kernel(Args a) {
     const float ln = logf(s);
     const long long tok = token_of(a, i);
     const float za = tok >= 0 && tok < a.vocab ? to_f(z[tok]) : NAN;
-    const Row r = row_terms(a, i, empty ? (za != za ? za : -INFINITY) : (za - m) - ln,
+    const Row r = row_terms(a, inputs_of(a, i),
+                            empty ? (za != za ? za : -INFINITY) : (za - m) - ln,
                             empty ? 0.f : ln - t / s, empty && za == za);
     if (GRAD) {
       // a token outside the vocabulary leaves c = NaN, and with it the row's gradient
@@ -666,16 +889,18 @@ __global__ void scalars_kernel(const double* partials, long long n, float kl, fl
 // -------------------------------------------------------------------------- the host
 // How a batch is run, by its vocabulary and type alone: short rows by groups of lanes,
 // longer ones by a warp, a CTA or a cluster each, whatever is longer by the loop.
-enum Kind { kGroup, kWarpRows, kSplit, kLoop };
+enum Kind { kTile, kGroup, kWarpRows, kSplit, kLoop };
 struct Plan {
   Kind kind;
-  int lanes, per_lane, rows_each;  // kGroup: L, E, R
+  int lanes, per_lane, rows_each;  // kGroup: L, E, R; kTile: per_lane = E
   int nv, threads, cluster;        // kWarpRows, kSplit
   long long blocks, n_partials;
   size_t partials_at, bytes;
 };
 
 constexpr int kShort = 512;
+constexpr long long kManyRows = 16384;
+constexpr long long kFewCtas = 148;
 
 int check(const swarp_policy_t* p) {
   if (!p || p->rows < 0 || p->vocab < 1 || p->vocab > 0x7fffffffll) return SWARP_ERR_INVALID_ARG;
@@ -689,7 +914,14 @@ Plan plan_of(const swarp_policy_t* p) {
   const long long V = p->vocab, rows = p->rows;
   const long long vecs = V / (p->dtype == SWARP_F32 ? 4 : 8);
   auto at_most = [&](long long n, long long cap) { return n < 1 ? 1 : n < cap ? n : cap; };
-  if (V <= kShort) {
+  const bool adjacent = p->inner == rows && p->stride_inner == V &&
+                        reinterpret_cast<uintptr_t>(p->logits) % 16 == 0 &&
+                        reinterpret_cast<uintptr_t>(p->grad) % 16 == 0;
+  if (V <= 32 && adjacent && rows >= kManyRows) {
+    q.kind = kTile;
+    q.per_lane = static_cast<int>((V + 7) / 8 * 8);
+    q.blocks = q.n_partials = at_most((rows + kTileRows - 1) / kTileRows, 148 * 8);
+  } else if (V <= kShort) {
     q.kind = kGroup;
     q.lanes = V <= 4 ? 1 : V <= 8 ? 2 : V <= 16 ? 4 : V <= 32 ? 8 : V <= 64 ? 16 : 32;
     q.per_lane = static_cast<int>((V + q.lanes - 1) / q.lanes);
@@ -703,23 +935,25 @@ Plan plan_of(const swarp_policy_t* p) {
     q.kind = kWarpRows;
     q.threads = 32, q.cluster = 1;
     q.nv = vecs <= 32 * 4 ? 4 : vecs <= 32 * 8 ? 8 : 16;
-    q.blocks = at_most((rows + 7) / 8, 148 * 8);
+    q.blocks = at_most((rows + 7) / 8, 148 * split_resident(32, q.nv));
     q.n_partials = q.blocks;
-  } else if (vecs <= 512ll * 8 * 8) {
+  } else if (vecs <= 256ll * 16 * 8) {
     q.kind = kSplit;
-    q.nv = vecs <= 256 * 4 ? 4 : 8;
-    q.threads = vecs <= 256ll * 8 * 8 ? 256 : 512;
+    q.nv = vecs <= 256 * 4 ? 4 : vecs <= 256 * 8 ? 8 : 16;
+    q.threads = 256;
     q.cluster = 1;
     while (vecs > static_cast<long long>(q.cluster) * q.threads * q.nv) q.cluster *= 2;
-    const long long clusters = at_most(rows, 148ll * 4 * 256 / q.threads / q.cluster);
-    q.blocks = clusters * q.cluster;
-    q.n_partials = clusters;
+    if (q.nv == 16 && q.cluster < 8 && rows * q.cluster <= kFewCtas) q.nv = 8, q.cluster *= 2;
+    // clusters; a launch may have fewer, as many as the device holds at once
+    q.n_partials = at_most(rows, 148ll * split_resident(q.threads, q.nv) / q.cluster);
+    q.blocks = q.n_partials * q.cluster;
   } else {
     q.kind = kLoop;
     q.blocks = q.n_partials = at_most(rows, kLoopMaxBlocks);
   }
   q.partials_at = align256(kCountBlocks * sizeof(long long));
-  q.bytes = q.partials_at + align256(sizeof(double) * 4 * q.n_partials);
+  // the same for every kind, so that it does not depend on the addresses
+  q.bytes = q.partials_at + align256(sizeof(double) * 4 * at_most(rows, kLoopMaxBlocks));
   return q;
 }
 
@@ -731,13 +965,19 @@ template <typename T, int L, int E, int R> int launch_group(const Args& a, const
   return launch_status();
 }
 
-template <typename T, int NV, int THREADS, int C> int launch_split(const Args& a, const Plan& q,
+template <typename T, int E> int launch_tile(const Args& a, const Plan& q, cudaStream_t st) {
+  const unsigned n = static_cast<unsigned>(q.blocks);
+  if (a.grad) policy_tile_kernel<T, E, true><<<n, kTileRows, 0, st>>>(a);
+  else policy_tile_kernel<T, E, false><<<n, kTileRows, 0, st>>>(a);
+  return launch_status();
+}
+
+template <typename T, int NV, int THREADS, int C> int launch_split(const Args& a, Plan& q,
                                                                    cudaStream_t st) {
   auto* f = a.grad ? policy_split_kernel<T, NV, THREADS, C, true>
                    : policy_split_kernel<T, NV, THREADS, C, false>;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(q.blocks));
-  cfg.blockDim = dim3(THREADS == 32 ? 256 : THREADS);
+  cfg.blockDim = dim3(split_block(THREADS));
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -745,10 +985,30 @@ template <typename T, int NV, int THREADS, int C> int launch_split(const Args& a
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = C > 1 ? 1 : 0;
+  cfg.gridDim = dim3(static_cast<unsigned>(q.blocks));
+  if (C > 1) {
+    // clusters that wait for others to end would double the time: rows are dealt out evenly
+    static std::atomic<int> resident[2];
+    int n = resident[a.grad != nullptr].load(std::memory_order_relaxed);
+    if (n == 0) {
+      if (cudaOccupancyMaxActiveClusters(&n, f, &cfg) != cudaSuccess || n < 1)
+        return SWARP_ERR_CUDA;
+      resident[a.grad != nullptr].store(n, std::memory_order_relaxed);
+    }
+    if (q.n_partials > n) {
+      q.n_partials = n;
+      cfg.gridDim.x = static_cast<unsigned>(n * C);
+    }
+  }
   return cudaLaunchKernelEx(&cfg, f, a) == cudaSuccess ? launch_status() : SWARP_ERR_CUDA;
 }
 
-template <typename T> int run_typed(const Args& a, const Plan& q, cudaStream_t st) {
+template <typename T> int run_typed(const Args& a, Plan& q, cudaStream_t st) {
+  if (q.kind == kTile)
+    return q.per_lane == 8    ? launch_tile<T, 8>(a, q, st)
+           : q.per_lane == 16 ? launch_tile<T, 16>(a, q, st)
+           : q.per_lane == 24 ? launch_tile<T, 24>(a, q, st)
+                              : launch_tile<T, 32>(a, q, st);
   if (q.kind == kGroup) {
     switch (q.lanes) {
       case 1: return launch_group<T, 1, 4, 1>(a, q, st);
@@ -772,12 +1032,16 @@ template <typename T> int run_typed(const Args& a, const Plan& q, cudaStream_t s
            : q.nv == 8 ? launch_split<T, 8, 32, 1>(a, q, st)
                        : launch_split<T, 16, 32, 1>(a, q, st);
   if (q.kind == kSplit) {
-    if (q.threads == 512) return launch_split<T, 8, 512, 8>(a, q, st);
     if (q.nv == 4) return launch_split<T, 4, 256, 1>(a, q, st);
-    return q.cluster == 1   ? launch_split<T, 8, 256, 1>(a, q, st)
-           : q.cluster == 2 ? launch_split<T, 8, 256, 2>(a, q, st)
-           : q.cluster == 4 ? launch_split<T, 8, 256, 4>(a, q, st)
-                            : launch_split<T, 8, 256, 8>(a, q, st);
+    if (q.nv == 8)
+      return q.cluster == 1   ? launch_split<T, 8, 256, 1>(a, q, st)
+             : q.cluster == 2 ? launch_split<T, 8, 256, 2>(a, q, st)
+             : q.cluster == 4 ? launch_split<T, 8, 256, 4>(a, q, st)
+                              : launch_split<T, 8, 256, 8>(a, q, st);
+    return q.cluster == 1   ? launch_split<T, 16, 256, 1>(a, q, st)
+           : q.cluster == 2 ? launch_split<T, 16, 256, 2>(a, q, st)
+           : q.cluster == 4 ? launch_split<T, 16, 256, 4>(a, q, st)
+                            : launch_split<T, 16, 256, 8>(a, q, st);
   }
   const unsigned n = static_cast<unsigned>(q.blocks);
   if (a.grad) policy_loop_kernel<T, true><<<n, kLoopThreads, 0, st>>>(a);
@@ -796,7 +1060,7 @@ int run(const swarp_policy_t* p, Call call, const float* cotangent, int skip_uni
   if (call != kGrad && some && (!p->logp || !p->entropy)) return SWARP_ERR_INVALID_ARG;
   if (loss && (!p->loss || !p->stats)) return SWARP_ERR_INVALID_ARG;
   if (call == kGrad && (!cotangent || (some && !p->grad))) return SWARP_ERR_INVALID_ARG;
-  const Plan q = plan_of(p);
+  Plan q = plan_of(p);
   if (!workspace || workspace_bytes < q.bytes) return SWARP_ERR_WORKSPACE;
   char* ws = static_cast<char*>(workspace);
   Args a{};
