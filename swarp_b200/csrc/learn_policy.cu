@@ -19,6 +19,7 @@ constexpr int kCountBlocks = 64;
 constexpr int kLoopThreads = 256;
 constexpr int kLoopMaxBlocks = 148 * 8;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
 struct Args {
   const void* logits;
@@ -447,16 +448,30 @@ template <> struct Vec<__half> {
   }
 };
 
-// A part of a row: the maximum of its logits, and its sums of e^x and e^x x with x counted
-// from that maximum (from 0 where all are -inf).
+// A part of a row: the maximum m of its logits, and with x2 = (z - m) log2 e its sums of 2^x2
+// and 2^x2 x2. The exponent is one fused operation, z log2 e - m2 with m2 = log2 e m rounded
+// once: all x2 of a part are then off by the same amount, and parts are joined by the
+// difference of their m2, so the row's sums and its p = 2^x2 / S stay consistent to the last
+// bit. Where log2 e m would come near the end of the range (a row of the type's lowest value,
+// say) x2 is formed from z - m instead; between the two kinds of parts the difference is so
+// large that nothing remains of the lower.
 struct Part {
   float m, s, t;
 };
+__device__ __forceinline__ bool ordinary(float m) { return fabsf(m) < 1e38f; }
 __device__ __forceinline__ float origin(float m) { return m == -INFINITY ? 0.f : m; }
+// m2, rounded as such (not contracted into what it is added to)
+__device__ __forceinline__ float scaled(float m) { return __fmul_rn(m, kLog2e); }
+// x2 of z, for a part that is not ordinary or that holds -inf (2^x2 x2 is to be 0 there)
+__device__ __forceinline__ float careful(float z, float m) {
+  const float x = ordinary(m) ? fmaf(z, kLog2e, -scaled(m)) : (z - origin(m)) * kLog2e;
+  return max_nan(x, -1e4f);
+}
 // p with its sums on the maximum `top`, in place of its own
 __device__ __forceinline__ void onto(Part& p, float top) {
-  const float d = max_nan(p.m - origin(top), -1e4f);  // a part of nothing: its sums are 0
-  const float f = exp2_fast(d * kLog2e);
+  const float d = max_nan(ordinary(top) ? __fsub_rn(scaled(p.m), scaled(top))
+                                        : (p.m - origin(top)) * kLog2e, -1e4f);
+  const float f = exp2_fast(d);
   p.t = fmaf(p.s, d, p.t) * f;
   p.s *= f;
   p.m = top;
@@ -622,8 +637,8 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS, 
       for (int k = 0; k < NV; ++k)
         if (k * kAllThreads + warp_at < cut.vecs) p.m = Vec<T>::most(q[k], p.m);
       {
-        const float o = origin(p.m);
-        auto sum = [&](auto bounded) {
+        const float m = p.m, m2 = -scaled(m);
+        auto sum = [&](auto care) {
           float s[2] = {0.f, 0.f}, t[2] = {0.f, 0.f};
 #pragma unroll
           for (int k = 0; k < NV; ++k)
@@ -631,20 +646,24 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS, 
 #pragma unroll
               for (int h = 0; h < N / 2; ++h) {
                 float2 x = Vec<T>::pair(q[k], h);
-                x.x -= o, x.y -= o;
-                if (decltype(bounded)::value) x.x = max_nan(x.x, -1e4f), x.y = max_nan(x.y, -1e4f);
-                const float e0 = exp2_fast(x.x * kLog2e), e1 = exp2_fast(x.y * kLog2e);
+                if (decltype(care)::value) {
+                  x.x = careful(x.x, m), x.y = careful(x.y, m);
+                } else {
+                  x.x = fmaf(x.x, kLog2e, m2), x.y = fmaf(x.y, kLog2e, m2);
+                }
+                const float e0 = exp2_fast(x.x), e1 = exp2_fast(x.y);
                 s[0] += e0, s[1] += e1;
                 t[0] = fmaf(e0, x.x, t[0]), t[1] = fmaf(e1, x.y, t[1]);
               }
             }
-          const float x = max_nan(ze - o, -1e4f), e = exp2_fast(x * kLog2e);
+          const float x = careful(ze, m), e = exp2_fast(x);
           p.s = s[0] + s[1] + e;
           p.t = fmaf(e, x, t[0] + t[1]);
         };
-        if (!low) sum(std::false_type{});
-        // 0 times -inf: again with x bounded below, and so from now on
-        if (low || p.t != p.t) low = true, sum(std::true_type{});
+        const bool plain = !low && ordinary(m);
+        if (plain) sum(std::false_type{});
+        // 0 times -inf: again with care, and so from now on
+        if (!plain || p.t != p.t) low = true, sum(std::true_type{});
       }
       // the next row, and what can be asked of it already
       const long long i2 = admitted(i + step);
@@ -698,21 +717,24 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS, 
         ++turn;
       }
       const bool empty = p.m == -INFINITY;
-      const float m = origin(p.m);
-      const float ln = empty ? 0.f : __logf(p.s), inv = empty ? 0.f : __fdividef(1.f, p.s);
-      const Row r = row_terms(a, in, empty ? (za != za ? za : -INFINITY) : (za - m) - ln,
-                              ln - p.t * inv, empty && za == za);
+      const float m = p.m, log2s = empty ? 0.f : __log2f(p.s);
+      const float inv = empty ? 0.f : __fdividef(1.f, p.s);
+      // a barred token has probability 0, but one in a row of nothing else, or outside, has
+      // the logit itself
+      const float xa = za == -INFINITY || za != za ? za : careful(za, m) - log2s;
+      const Row r = row_terms(a, in, xa * kLn2, (log2s - p.t * inv) * kLn2, empty && za == za);
       if (at == 0) {
         if (a.logp) a.logp[i] = r.lp, a.entropy[i] = r.H;
         sums[0] += r.pg, sums[1] += r.k3, sums[2] += r.H, sums[3] += r.cut;
       }
       if (GRAD) {
         const float c = wg * r.c, eta = wg * a.ent;
-        const float k0 = inv * (eta * (r.H - ln) - c), k1 = inv * eta;
+        const float k0 = inv * (eta * (r.H - log2s * kLn2) - c), k1 = inv * eta * kLn2;
+        const float m2 = -scaled(m);
         T* g = static_cast<T*>(a.grad) + i * V;
         uint4* gv = reinterpret_cast<uint4*>(g + cut.head);
         const bool same_phase = (reinterpret_cast<uintptr_t>(gv) & 15) == 0;
-        // kind 0: no entropy term; 1: with it; 2: with it, x bounded
+        // kind 0: no entropy term; 1: with it; 2: either, with care
         auto write = [&](auto kind) {
           constexpr int kKind = decltype(kind)::value;
 #pragma unroll
@@ -723,9 +745,12 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS, 
 #pragma unroll
               for (int h = 0; h < N / 2; ++h) {
                 float2 x = Vec<T>::pair(q[k], h);
-                x.x -= m, x.y -= m;
-                if (kKind == 2) x.x = max_nan(x.x, -1e4f), x.y = max_nan(x.y, -1e4f);
-                const float e0 = exp2_fast(x.x * kLog2e), e1 = exp2_fast(x.y * kLog2e);
+                if (kKind == 2) {
+                  x.x = careful(x.x, m), x.y = careful(x.y, m);
+                } else {
+                  x.x = fmaf(x.x, kLog2e, m2), x.y = fmaf(x.y, kLog2e, m2);
+                }
+                const float e0 = exp2_fast(x.x), e1 = exp2_fast(x.y);
                 Vec<T>::set(out, h, kKind == 0 ? make_float2(e0 * k0, e1 * k0)
                                                : make_float2(e0 * fmaf(k1, x.x, k0),
                                                              e1 * fmaf(k1, x.y, k0)));
@@ -743,12 +768,13 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS, 
             q[k] = fetch(cut2, k);
           }
         };
-        if (a.ent == 0.f) write(std::integral_constant<int, 0>{});
-        else if (!low) write(std::integral_constant<int, 1>{});
-        else write(std::integral_constant<int, 2>{});
+        // without the entropy term a logit of -inf needs no care
+        if (!ordinary(m) || (low && a.ent != 0.f)) write(std::integral_constant<int, 2>{});
+        else if (a.ent == 0.f) write(std::integral_constant<int, 0>{});
+        else write(std::integral_constant<int, 1>{});
         auto alone = [&](float zj) {
-          const float x = max_nan(zj - m, -1e4f);
-          return exp2_fast(x * kLog2e) * fmaf(k1, x, k0);
+          const float x = careful(zj, m);
+          return exp2_fast(x) * fmaf(k1, x, k0);
         };
         if (cut.edge >= 0) g[cut.edge] = from_f<T>(alone(ze));
         // the token's own place again, by the thread that has just written it
@@ -900,7 +926,6 @@ struct Plan {
 
 constexpr int kShort = 512;
 constexpr long long kManyRows = 16384;
-constexpr long long kFewCtas = 148;
 
 int check(const swarp_policy_t* p) {
   if (!p || p->rows < 0 || p->vocab < 1 || p->vocab > 0x7fffffffll) return SWARP_ERR_INVALID_ARG;
@@ -943,7 +968,6 @@ Plan plan_of(const swarp_policy_t* p) {
     q.threads = 256;
     q.cluster = 1;
     while (vecs > static_cast<long long>(q.cluster) * q.threads * q.nv) q.cluster *= 2;
-    if (q.nv == 16 && q.cluster < 8 && rows * q.cluster <= kFewCtas) q.nv = 8, q.cluster *= 2;
     // clusters; a launch may have fewer, as many as the device holds at once
     q.n_partials = at_most(rows, 148ll * split_resident(q.threads, q.nv) / q.cluster);
     q.blocks = q.n_partials * q.cluster;
@@ -1033,11 +1057,7 @@ template <typename T> int run_typed(const Args& a, Plan& q, cudaStream_t st) {
                        : launch_split<T, 16, 32, 1>(a, q, st);
   if (q.kind == kSplit) {
     if (q.nv == 4) return launch_split<T, 4, 256, 1>(a, q, st);
-    if (q.nv == 8)
-      return q.cluster == 1   ? launch_split<T, 8, 256, 1>(a, q, st)
-             : q.cluster == 2 ? launch_split<T, 8, 256, 2>(a, q, st)
-             : q.cluster == 4 ? launch_split<T, 8, 256, 4>(a, q, st)
-                              : launch_split<T, 8, 256, 8>(a, q, st);
+    if (q.nv == 8) return launch_split<T, 8, 256, 1>(a, q, st);
     return q.cluster == 1   ? launch_split<T, 16, 256, 1>(a, q, st)
            : q.cluster == 2 ? launch_split<T, 16, 256, 2>(a, q, st)
            : q.cluster == 4 ? launch_split<T, 16, 256, 4>(a, q, st)
