@@ -184,23 +184,38 @@ __device__ __forceinline__ uint32_t code_of(uint2 q, int k) {
 
 // ------------------------------------------------------------------- sums of squares
 // Eight squares in float, then on in double: the norm is good to float rounding at any size.
+// Four chunks at a time, so that enough loads are in flight.
 template <typename T, int CAP>
 __global__ void __launch_bounds__(kThreads)
     norm_kernel(const __grid_constant__ Table<CAP> tab, double* partials) {
+  constexpr int kAtOnce = 4;
   __shared__ double part[kThreads / 32];
   double s = 0;
-  for (int b = blockIdx.x; b < tab.first_chunk[tab.n]; b += gridDim.x) {
-    const int k = tensor_of(tab, b);
-    const long long i =
-        static_cast<long long>(b - tab.first_chunk[k]) * kChunk + threadIdx.x * 8ll;
-    const long long left = static_cast<long long>(tab.t[k].n) - i;
-    if (left <= 0) continue;
-    float g[8], q = 0.f;
-    load8(static_cast<const T*>(tab.t[k].grad) + i, g, tab.vectors[k] && left >= 8,
-          static_cast<int>(min(left, 8ll)));
+  const int chunks = tab.first_chunk[tab.n];
+  for (int b0 = blockIdx.x * kAtOnce; b0 < chunks; b0 += gridDim.x * kAtOnce) {
+    float g[kAtOnce][8];
+    int k = tensor_of(tab, b0);
 #pragma unroll
-    for (int h = 0; h < 8; ++h) q = fmaf(g[h], g[h], q);
-    s += q;
+    for (int c = 0; c < kAtOnce; ++c) {
+      const int b = b0 + c;
+#pragma unroll
+      for (int h = 0; h < 8; ++h) g[c][h] = 0.f;
+      if (b >= chunks) continue;
+      while (tab.first_chunk[k + 1] <= b) ++k;
+      const long long i =
+          static_cast<long long>(b - tab.first_chunk[k]) * kChunk + threadIdx.x * 8ll;
+      const long long left = static_cast<long long>(tab.t[k].n) - i;
+      if (left > 0)
+        load8(static_cast<const T*>(tab.t[k].grad) + i, g[c], tab.vectors[k] && left >= 8,
+              static_cast<int>(min(left, 8ll)));
+    }
+#pragma unroll
+    for (int c = 0; c < kAtOnce; ++c) {
+      float q = 0.f;
+#pragma unroll
+      for (int h = 0; h < 8; ++h) q = fmaf(g[c][h], g[c][h], q);
+      s += q;
+    }
   }
   s = warp_sum(s);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;

@@ -35,28 +35,52 @@ __device__ __forceinline__ Step<T> load_step(const Args<T>& a, long long t, long
 }
 
 // ------------------------------------------------------------------ many columns
-// One thread per column walks the steps backwards, kAhead steps' loads in flight.
-template <typename T> __global__ void __launch_bounds__(256) gae_columns_kernel(Args<T> a) {
-  constexpr int kAhead = 8;
-  const long long j = blockIdx.x * 256ll + threadIdx.x;
+// One thread per W columns (one 16-byte access, or one element) walks the steps backwards,
+// with the loads of kAhead steps in flight.
+template <typename T, int W> struct alignas(W * sizeof(T)) Pack {
+  T x[W];
+};
+constexpr int kColumnThreads = 64;
+
+template <typename T, int W, bool NEXT>
+__global__ void __launch_bounds__(kColumnThreads) gae_columns_kernel(Args<T> a) {
+  constexpr int kAhead = W == 1 ? 8 : 4;
+  using P = Pack<T, W>;
+  const long long j = (blockIdx.x * static_cast<long long>(kColumnThreads) + threadIdx.x) * W;
   if (j >= a.columns) return;
-  const long long f = j / a.per_flag;
-  T A = 0, after = a.next ? T(0) : a.last[j];
+  const long long f = j / a.per_flag;  // W columns share their flags
+  P A{}, after{};
+  if (!NEXT) after = *reinterpret_cast<const P*>(a.last + j);
   for (long long t = a.steps; t > 0; t -= kAhead) {
-    Step<T> s[kAhead];
+    P r[kAhead], v[kAhead], next[NEXT ? kAhead : 1];
+    bool term[kAhead], stop[kAhead];
+    const int n = static_cast<int>(min(t, static_cast<long long>(kAhead)));
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-      if (t - 1 - k >= 0) s[k] = load_step(a, t - 1 - k, j, f);
+      if (k < n) {
+        const long long at = (t - 1 - k) * a.columns + j, g = (t - 1 - k) * a.flags + f;
+        r[k] = *reinterpret_cast<const P*>(a.r + at);
+        v[k] = *reinterpret_cast<const P*>(a.v + at);
+        if (NEXT) next[NEXT ? k : 0] = *reinterpret_cast<const P*>(a.next + at);
+        term[k] = a.term && a.term[g];
+        stop[k] = term[k] || (a.trunc && a.trunc[g]) || a.decay == T(0);
+      }
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (t - 1 - k < 0) break;
-      const T d = s[k].r + (s[k].term ? T(0) : a.gamma * (a.next ? s[k].next : after)) - s[k].v;
-      A = s[k].stop ? d : d + a.decay * A;
-      const long long at = (t - 1 - k) * a.columns + j;
-      a.adv[at] = A;
-      a.ret[at] = A + s[k].v;
-      after = s[k].v;
-    }
+    for (int k = 0; k < kAhead; ++k)
+      if (k < n) {
+        const long long at = (t - 1 - k) * a.columns + j;
+        P ret;
+#pragma unroll
+        for (int c = 0; c < W; ++c) {
+          const T follow = NEXT ? next[NEXT ? k : 0].x[c] : after.x[c];
+          const T d = r[k].x[c] + (term[k] ? T(0) : a.gamma * follow) - v[k].x[c];
+          A.x[c] = stop[k] ? d : d + a.decay * A.x[c];
+          ret.x[c] = A.x[c] + v[k].x[c];
+        }
+        *reinterpret_cast<P*>(a.adv + at) = A;
+        *reinterpret_cast<P*>(a.ret + at) = ret;
+        after = v[k];
+      }
   }
 }
 
@@ -193,7 +217,19 @@ template <typename T> int run(const swarp_gae_t* g, const Plan& q, void* ws, cud
     gae_segments_kernel<T, true><<<grid, kCtaThreads, 0, st>>>(a, q.tile, q.segments, maps);
     return launch_status();
   }
-  gae_columns_kernel<T><<<(unsigned)((g->columns + 255) / 256), 256, 0, st>>>(a);
+  constexpr int W = 16 / sizeof(T);
+  // whole packs that share a flag, all of them aligned
+  const bool flagged = a.term || a.trunc;
+  bool packs = a.columns % W == 0 && (!flagged || a.per_flag % W == 0);
+  for (const void* p : {static_cast<const void*>(a.r), static_cast<const void*>(a.v),
+                        static_cast<const void*>(a.next), static_cast<const void*>(a.last),
+                        static_cast<const void*>(a.adv), static_cast<const void*>(a.ret)})
+    packs = packs && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  const long long threads = packs ? a.columns / W : a.columns;
+  const unsigned blocks = static_cast<unsigned>((threads + kColumnThreads - 1) / kColumnThreads);
+  auto* kernel = packs ? (a.next ? gae_columns_kernel<T, W, true> : gae_columns_kernel<T, W, false>)
+                       : (a.next ? gae_columns_kernel<T, 1, true> : gae_columns_kernel<T, 1, false>);
+  kernel<<<blocks, kColumnThreads, 0, st>>>(a);
   return launch_status();
 }
 

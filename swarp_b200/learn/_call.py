@@ -12,6 +12,21 @@ from swarp_b200 import _lib
 DTYPES = {torch.float32: 0, torch.float64: 1, torch.bfloat16: 2, torch.float16: 3}
 
 _HERE = contextlib.nullcontext()
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_lib_loaded = None
+
+
+def library():
+    """The loaded library; its checks for a device and a build run on the first call."""
+    global _lib_loaded
+    if _lib_loaded is None:
+        _lib_loaded = _lib.load()
+    return _lib_loaded
+
+
+def stream(device: torch.device) -> int:
+    """torch's current stream of ``device``, without a Stream object where torch has a way."""
+    return _raw_stream(device.index) if _raw_stream else _lib.stream_ptr(device)
 
 
 def on_device(device: torch.device):
@@ -19,14 +34,14 @@ def on_device(device: torch.device):
     return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
-def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+def workspace(nbytes: int, like: torch.Tensor) -> torch.Tensor:
+    return like.new_empty(nbytes, dtype=torch.uint8)
 
 
 def require_cuda(t: torch.Tensor, name: str) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise RuntimeError(f"{name} is on {t.device}: swarp_b200 runs on a CUDA device only "
                            "(no CPU path)")
 
@@ -42,7 +57,7 @@ def like(t: torch.Tensor, name: str, shape, dtypes, device) -> torch.Tensor:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def constant(t: torch.Tensor | None, name: str) -> None:
@@ -51,4 +66,5 @@ def constant(t: torch.Tensor | None, name: str) -> None:
         raise ValueError(f"{name} requires grad, but no gradient flows to it here: detach it")
 
 
-__all__ = ["DTYPES", "constant", "like", "on_device", "require_cuda", "workspace", "_lib"]
+__all__ = ["DTYPES", "constant", "library", "like", "on_device", "require_cuda", "stream",
+           "workspace"]

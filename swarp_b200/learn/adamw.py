@@ -18,13 +18,16 @@ number, and with it the bias corrections and the random bits, that it was captur
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 from collections.abc import Sequence
+from itertools import chain
+from operator import attrgetter
 from typing import Any, NamedTuple
 
 import torch
 
 from swarp_b200 import _lib
-from swarp_b200.learn._call import DTYPES, on_device, require_cuda
+from swarp_b200.learn._call import DTYPES, library, on_device, require_cuda, stream
 
 _PARAM_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 BLOCK = 256  # SWARP_MOMENT_BLOCK
@@ -57,11 +60,11 @@ class Moment8(NamedTuple):
         n, device = self.codes.numel(), self.codes.device
         _check_moment8(self, "moment", n, device)
         out = torch.empty(n, dtype=dtype, device=device)
-        lib = _lib.load()
+        lib = library()
         with on_device(device):
             _lib.check(lib.swarp_moment8_values(
                 self.codes.data_ptr(), self.exponents.data_ptr(), n, self.signed, DTYPES[dtype],
-                out.data_ptr(), _lib.stream_ptr(device)), "swarp_moment8_values")
+                out.data_ptr(), stream(device)), "swarp_moment8_values")
         return out
 
 
@@ -73,16 +76,37 @@ def _check_moment8(m: Moment8, name: str, n: int, device) -> None:
                              f"{t.dtype} {tuple(t.shape)} on {t.device}")
 
 
+# a step may have hundreds of tensors: their properties are read by C loops
+_numel, _ptr, _contiguous, _device = (torch.Tensor.numel, torch.Tensor.data_ptr,
+                                      torch.Tensor.is_contiguous, torch.Tensor.get_device)
+_dtype, _shape = attrgetter("dtype"), attrgetter("shape")
+
+
 def _same(ts, name, sizes, dtype, device):
     """The addresses of ``ts``, once each has its parameter's size and is contiguous."""
     if len(ts) != len(sizes):
         raise ValueError(f"{len(sizes)} params but {len(ts)} {name}")
-    for i, (t, n) in enumerate(zip(ts, sizes)):
-        if t.dtype != dtype or t.numel() != n or t.device != device or not t.is_contiguous():
-            kind = TypeError if t.dtype != dtype else ValueError
-            raise kind(f"{name}[{i}] must be {n} contiguous {dtype} elements on {device}, got "
-                       f"{t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
-    return [t.data_ptr() for t in ts]
+    if not (list(map(_numel, ts)) == sizes and set(map(_dtype, ts)) == {dtype}
+            and set(map(_device, ts)) == {device.index} and all(map(_contiguous, ts))):
+        for i, (t, n) in enumerate(zip(ts, sizes)):
+            if t.dtype != dtype or t.numel() != n or t.device != device or not t.is_contiguous():
+                kind = TypeError if t.dtype != dtype else ValueError
+                raise kind(f"{name}[{i}] must be {n} contiguous {dtype} elements on {device}, "
+                           f"got {t.dtype} {tuple(t.shape)} with strides {t.stride()} on "
+                           f"{t.device}")
+    return list(map(_ptr, ts))
+
+
+def _same8(ms, name, sizes, blocks, signed, device):
+    """The addresses of the codes and exponents of 8-bit moments."""
+    if len(ms) != len(sizes):
+        raise ValueError(f"{len(sizes)} params but {len(ms)} {name}")
+    for i, x in enumerate(ms):
+        if not isinstance(x, Moment8) or x.signed != signed:
+            raise TypeError(f"{name}[{i}] must be a Moment8 with signed={signed}")
+    codes, exps = [x.codes for x in ms], [x.exponents for x in ms]
+    return (_same(codes, name + " codes", sizes, torch.uint8, device),
+            _same(exps, name + " exponents", blocks, torch.uint8, device))
 
 
 class _Tensors:
@@ -96,15 +120,15 @@ class _Tensors:
         self.device, self.dtype = params[0].device, params[0].dtype
         if self.dtype not in _PARAM_DTYPES:
             raise TypeError(f"params dtype {self.dtype}: want float32, bfloat16 or float16")
-        sizes = [p.numel() for p in params]
+        sizes = list(map(_numel, params))
         zero = [0] * n
         p = _same(params, "params", sizes, self.dtype, self.device)
-        # a gradient may be in another memory order than its parameter's
         g = _same(grads, "grads", sizes, self.dtype, self.device)
-        for i, (x, y) in enumerate(zip(params, grads)):
-            if x.shape != y.shape:
-                raise ValueError(f"grads[{i}] has shape {tuple(y.shape)}, its parameter "
-                                 f"{tuple(x.shape)}")
+        if list(map(_shape, params)) != list(map(_shape, grads)):
+            for i, (x, y) in enumerate(zip(params, grads)):
+                if x.shape != y.shape:
+                    raise ValueError(f"grads[{i}] has shape {tuple(y.shape)}, its parameter "
+                                     f"{tuple(x.shape)}")
         if self.dtype == torch.float32:
             if masters is not None:
                 raise ValueError("masters are for 16-bit parameters")
@@ -113,30 +137,23 @@ class _Tensors:
             raise ValueError(f"{self.dtype} parameters need float32 masters")
         else:
             w = _same(masters, "masters", sizes, torch.float32, self.device)
-        self.bits = 8 if isinstance(exp_avg[0], Moment8) else 32
+        self.bits = 8 if len(exp_avg) and isinstance(exp_avg[0], Moment8) else 32
         if self.bits == 32:
             m = _same(exp_avg, "exp_avg", sizes, torch.float32, self.device)
             v = _same(exp_avg_sq, "exp_avg_sq", sizes, torch.float32, self.device)
             me = ve = zero
         else:
-            for ms, name, signed in ((exp_avg, "exp_avg", True),
-                                     (exp_avg_sq, "exp_avg_sq", False)):
-                if len(ms) != n:
-                    raise ValueError(f"{n} params but {len(ms)} {name}")
-                for i, (x, size) in enumerate(zip(ms, sizes)):
-                    if not isinstance(x, Moment8) or x.signed != signed:
-                        raise TypeError(f"{name}[{i}] must be a Moment8 with signed={signed}")
-                    _check_moment8(x, f"{name}[{i}]", size, self.device)
-            m, me = [x.codes.data_ptr() for x in exp_avg], [x.exponents.data_ptr() for x in exp_avg]
-            v, ve = ([x.codes.data_ptr() for x in exp_avg_sq],
-                     [x.exponents.data_ptr() for x in exp_avg_sq])
-        flat = [x for row in zip(sizes, p, g, w, m, v, me, ve) for x in row]
+            blocks = [-(-x // BLOCK) for x in sizes]
+            m, me = _same8(exp_avg, "exp_avg", sizes, blocks, True, self.device)
+            v, ve = _same8(exp_avg_sq, "exp_avg_sq", sizes, blocks, False, self.device)
         self.params, self.keep = params, grads  # until the launch has read their addresses
-        self.n, self.c = n, (C.c_uint64 * len(flat))(*flat)  # swarp_adamw_tensor_t[n]
+        # swarp_adamw_tensor_t[n], in 64-bit words
+        self.words = array("Q", chain.from_iterable(zip(sizes, p, g, w, m, v, me, ve)))
+        self.n, self.c = n, self.words.buffer_info()[0]
 
     def norm_partials(self, lib, out: torch.Tensor) -> None:
         _lib.check(lib.swarp_grad_norm_partials(DTYPES[self.dtype], self.c, self.n,
-                                                out.data_ptr(), _lib.stream_ptr(self.device)),
+                                                out.data_ptr(), stream(self.device)),
                    "swarp_grad_norm_partials")
 
     def step(self, lib, step, lr, betas, eps, weight_decay, seed, first, partials, max_norm,
@@ -146,7 +163,7 @@ class _Tensors:
                             0 if partials is None else partials.numel(), max_norm or 0.0,
                             _lib.ptr(norm))
         _lib.check(lib.swarp_adamw_step(C.byref(opt), self.c, self.n,
-                                        _lib.stream_ptr(self.device)), "swarp_adamw_step")
+                                        stream(self.device)), "swarp_adamw_step")
         # autograd must see that the parameters changed, as after torch's own in-place steps
         torch.autograd.graph.increment_version(self.params)
 
@@ -187,7 +204,7 @@ def adamw_step(
     their norm before that is returned (a float32 scalar on the device)."""
     _check_settings(step, lr, betas, eps, weight_decay, max_norm)
     ts = _Tensors(params, grads, exp_avg, exp_avg_sq, masters)
-    lib = _lib.load()
+    lib = library()
     partials = norm = None
     with on_device(ts.device):
         if max_norm is not None:
@@ -250,7 +267,7 @@ class AdamW(torch.optim.Optimizer):
                 index += 1
         if not sets:
             return loss
-        lib = _lib.load()
+        lib = library()
         made, device = [], None
         for (gi, dtype, dev, step), members in sets.items():
             if device is not None and dev != device:

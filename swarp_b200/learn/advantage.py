@@ -16,7 +16,16 @@ import math
 import torch
 
 from swarp_b200 import _lib
-from swarp_b200.learn._call import DTYPES, constant, like, on_device, require_cuda, workspace
+from swarp_b200.learn._call import (
+    DTYPES,
+    constant,
+    library,
+    like,
+    on_device,
+    require_cuda,
+    stream,
+    workspace,
+)
 
 _FLOATS = (torch.float32, torch.float64)
 _BOOL = (torch.bool,)
@@ -77,19 +86,18 @@ def gae(
         flags.append(t)
     columns = math.prod(shape[1:])
     per_flag = math.prod(shape[len(lead):]) if lead is not None else 1
-    adv = torch.empty(shape, dtype=dtype, device=device)
+    adv = torch.empty_like(r)
     ret = torch.empty_like(adv)
     if adv.numel() == 0:
         return adv, ret
     c = _lib.Gae(DTYPES[dtype], per_flag, shape[0], columns,
                  *(_lib.ptr(t) for t in (r, v, nxt, last, *flags)), gamma, lam, adv.data_ptr(),
                  ret.data_ptr())
-    lib = _lib.load()
+    lib = library()
     with on_device(device):
         n = lib.swarp_gae_workspace_bytes(C.byref(c))
-        ws = workspace(n, device) if n else None
-        _lib.check(lib.swarp_gae(C.byref(c), _lib.ptr(ws), n, _lib.stream_ptr(device)),
-                   "swarp_gae")
+        ws = workspace(n, r) if n else None
+        _lib.check(lib.swarp_gae(C.byref(c), _lib.ptr(ws), n, stream(device)), "swarp_gae")
     return adv, ret
 
 

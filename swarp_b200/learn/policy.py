@@ -19,10 +19,18 @@ import ctypes as C
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from swarp_b200 import _lib
-from swarp_b200.learn._call import DTYPES, constant, like, on_device, require_cuda, workspace
+from swarp_b200.learn._call import (
+    DTYPES,
+    constant,
+    library,
+    like,
+    on_device,
+    require_cuda,
+    stream,
+    workspace,
+)
 
 _LOGIT_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _TOKEN_DTYPES = (torch.int64, torch.int32)
@@ -69,7 +77,8 @@ def _rows(logits: torch.Tensor):
 
 
 class _Batch:
-    """Checked arguments as the C struct; holds the tensors that it points to."""
+    """Checked arguments as the C struct, and the tensors that it points to (``keep``, the
+    logits first)."""
 
     def __init__(self, logits, tokens, old_logp=None, advantages=None, ref_logp=None, mask=None,
                  clip_low=0.0, clip_high=0.0, kl_coef=0.0, entropy_coef=0.0, mean=True,
@@ -81,9 +90,9 @@ class _Batch:
             raise ValueError(f"logits must be [..., V] with V >= 1, got {tuple(logits.shape)}")
         self.shape = lead = logits.shape[:-1]
         self.device = device = logits.device
-        self.logits, self.rows, inner, outer_stride, inner_stride = _rows(logits)
-        self.tokens = like(tokens, "tokens", lead, _TOKEN_DTYPES, device)
-        keep = [self.logits, self.tokens]
+        rowed, rows, inner, outer_stride, inner_stride = _rows(logits)
+        tokens = like(tokens, "tokens", lead, _TOKEN_DTYPES, device)
+        self.keep = keep = [rowed, tokens]
         small = []
         for t, name, dtypes in ((old_logp, "old_logp", _F32), (advantages, "advantages", _F32),
                                 (ref_logp, "ref_logp", _F32), (mask, "mask", _BOOL)):
@@ -92,40 +101,39 @@ class _Batch:
                 t = like(t, name, lead, dtypes, device)
                 keep.append(t)
             small.append(None if t is None else t.data_ptr())
-        self.keep = keep
-        self.c = _lib.Policy(DTYPES[logits.dtype], self.tokens.dtype == torch.int64, self.rows,
+        self.c = _lib.Policy(DTYPES[logits.dtype], tokens.dtype == torch.int64, rows,
                              logits.shape[-1], inner, outer_stride, inner_stride,
-                             self.logits.data_ptr(), self.tokens.data_ptr(), *small, clip_low,
-                             clip_high, kl_coef, entropy_coef, mean, grad_scale)
+                             rowed.data_ptr(), tokens.data_ptr(), *small, clip_low, clip_high,
+                             kl_coef, entropy_coef, mean, grad_scale)
 
     def outputs(self):
-        logp = torch.empty(self.shape, dtype=torch.float32, device=self.device)
+        logp = self.keep[0].new_empty(self.shape, dtype=torch.float32)
         entropy = torch.empty_like(logp)
         self.c.logp, self.c.entropy = logp.data_ptr(), entropy.data_ptr()
         return logp, entropy
 
-    def new_grad(self):
-        grad = torch.empty((*self.shape, self.c.vocab), dtype=self.logits.dtype,
-                           device=self.device)
+    def new_grad(self, logits):
+        grad = (torch.empty_like(logits) if logits.is_contiguous() else
+                logits.new_empty((*self.shape, self.c.vocab)))
         self.c.grad = grad.data_ptr()
         return grad
 
-    def call(self, what: str, *args):
-        lib = _lib.load()
+    def call(self, what: str, on: torch.Tensor, *args):
+        lib = library()
         with on_device(self.device):
             ref = C.byref(self.c)
             n = lib.swarp_policy_workspace_bytes(ref)
-            ws = workspace(n, self.device)
-            _lib.check(getattr(lib, what)(ref, *args, ws.data_ptr(), n,
-                                          _lib.stream_ptr(self.device)), what)
+            ws = workspace(n, on)
+            rc = getattr(lib, what)(ref, *args, ws.data_ptr(), n, stream(self.device))
+        if rc:
+            _lib.check(rc, what)
 
     def loss(self, with_grad: bool):
         logp, entropy = self.outputs()
-        loss = torch.empty((), dtype=torch.float32, device=self.device)
-        stats = torch.empty(4, dtype=torch.float32, device=self.device)
+        loss, stats = logp.new_empty(()), logp.new_empty(4)
         self.c.loss, self.c.stats = loss.data_ptr(), stats.data_ptr()
-        grad = self.new_grad() if with_grad else None
-        self.call("swarp_policy_loss")
+        grad = self.new_grad(self.keep[0]) if with_grad else None
+        self.call("swarp_policy_loss", logp)
         return PolicyLoss(loss, logp, entropy, stats), grad
 
 
@@ -137,25 +145,27 @@ class _PolicyLossFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, batch):
-        out, grad = batch.loss(True)
-        ctx.batch, ctx.grad = batch, grad
-        ctx.save_for_backward(logits)  # only for its check against changes in place
+        out, ctx.grad = batch.loss(True)
+        # autograd alone keeps the inputs, so that a loss kept for the record frees them
+        ctx.save_for_backward(logits, *batch.keep)
+        batch.keep = None
+        ctx.batch = batch
         ctx.mark_non_differentiable(*out[1:])
         ctx.set_materialize_grads(False)
         return tuple(out)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_loss, *_):
         if g_loss is None:
             return None, None
-        ctx.saved_tensors
+        if torch.is_grad_enabled():
+            raise RuntimeError("policy_loss is differentiable once (create_graph is not supported)")
+        _, logits, *_ = held = ctx.saved_tensors  # noqa: F841  alive until the launch
         batch, grad, ctx.grad = ctx.batch, ctx.grad, None
         skip_unit = grad is not None
         if grad is None:  # a second backward of a retained graph: the buffer is gone
-            grad = batch.new_grad()
-        g_loss = g_loss.contiguous()
-        batch.call("swarp_policy_grad", g_loss.data_ptr(), int(skip_unit))
+            grad = batch.new_grad(logits)
+        batch.call("swarp_policy_grad", logits, g_loss.data_ptr(), int(skip_unit))
         return grad, None
 
 
@@ -244,7 +254,7 @@ def token_logp(logits: torch.Tensor, tokens: torch.Tensor) -> tuple[torch.Tensor
     constant(logits, "logits")
     b = _Batch(logits, tokens)
     out = b.outputs()
-    b.call("swarp_token_logp")
+    b.call("swarp_token_logp", out[0])
     return out
 
 
