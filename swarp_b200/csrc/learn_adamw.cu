@@ -8,6 +8,8 @@
 // 8-bit moments round up or down at random, without bias: to the nearest, an average that
 // moves by 1 - b2 = 0.1% a step would never leave a code 12.5% wide. Their new values are
 // formed with every rounding written out, so the codes depend on the inputs alone.
+#include <cuda_fp8.h>
+
 #include "learn.cuh"
 
 namespace swarp {
@@ -47,6 +49,14 @@ __host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
   return x ^ (x >> 16);
 }
 
+// the rest of mix(), after its first step
+__device__ __forceinline__ uint32_t mix_on(uint32_t x) {
+  x *= 0xE80B5AE5u;
+  x ^= x >> 15;
+  x *= 0xCB276749u;
+  return x ^ (x >> 16);
+}
+
 // the tensor of chunk b: the last whose first chunk is not beyond it
 template <int CAP> __device__ __forceinline__ int tensor_of(const Table<CAP>& tab, int b) {
   int lo = 0, hi = tab.n - 1;
@@ -56,6 +66,17 @@ template <int CAP> __device__ __forceinline__ int tensor_of(const Table<CAP>& ta
     else hi = mid - 1;
   }
   return lo;
+}
+
+// A CTA's run of chunks, and the tensor of its first
+struct Span {
+  int at, end, tensor;
+};
+template <int CAP> __device__ __forceinline__ Span span_of(const Table<CAP>& tab) {
+  const int chunks = tab.first_chunk[tab.n];
+  const int each = (chunks + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+  const int at = static_cast<int>(blockIdx.x) * each, end = min(at + each, chunks);
+  return Span{at, end, at < end ? tensor_of(tab, at) : 0};
 }
 
 // The gradients' scale, the same in every CTA: the partial sums added in a fixed order.
@@ -82,11 +103,16 @@ __device__ __forceinline__ float clip_scale(const Opt& o) {
 struct Elem {
   float p, m, v;
 };
-// to 1 ulp, subnormals included; the step's own size is good to 4 ulp then, of which the
-// parameter keeps a few parts in a thousand
+// sqrt(x) and 1 / x to 1 ulp where they are not subnormal: the step's own size is good to 4 ulp
+// then, of which the parameter keeps a few parts in a thousand
 __device__ __forceinline__ float sqrt_fast(float x) {
   float r;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 // The step of one element; m and v with every rounding written out.
@@ -94,31 +120,67 @@ __device__ __forceinline__ Elem adam(const Opt& o, float p, float g, float m, fl
   Elem e;
   e.m = __fadd_rn(__fmul_rn(m, o.b1), __fmul_rn(g, o.a1));
   e.v = __fadd_rn(__fmul_rn(v, o.b2), __fmul_rn(__fmul_rn(g, o.a2), g));
-  e.p = p * o.keep - o.rate * __fdividef(e.m, sqrt_fast(e.v) * o.root2 + o.eps);
+  // a subnormal v counts as 2^-126, whose root is 1e-19: only a smaller eps would notice
+  const float root = sqrt_fast(max_nan(e.v, 1.17549435e-38f));
+  e.p = p * o.keep - o.rate * (e.m * rcp_fast(root * o.root2 + o.eps));
   return e;
 }
 
+// A code as the float that it stands for; byte k of w.
+__device__ __forceinline__ uint32_t byte_of(uint32_t w, int k) {
+  return __byte_perm(w, 0, 0x4440 | k);  // the byte alone
+}
 __device__ __forceinline__ float decode_m(uint32_t code, int exp) {
   const uint32_t f = code & 127u;
   const uint32_t bits = ((f + 8u * exp - 112u) << 20) | ((code & 128u) << 24);
   return f ? __uint_as_float(bits) : 0.f;
 }
+// the same for a pair of codes of a block with an ordinary exponent: f is then a float of four
+// exponent and three mantissa bits, which the hardware knows, times 2^(exp - 134)
+__device__ __forceinline__ bool ordinary_exp(int exp) { return exp >= 14 && exp < 255; }
+__device__ __forceinline__ float2 decode_m2(uint32_t codes, float scale) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes),
+                                                   __NV_E4M3);
+  const float2 f = __half22float2(__half2(h));
+  return make_float2(f.x * scale, f.y * scale);
+}
 __device__ __forceinline__ float decode_v(uint32_t code, int exp) {
-  return code ? __uint_as_float((code + 8u * exp - 247u) << 20) : 0.f;
+  return code ? __uint_as_float((code << 20) + ((8u * exp - 247u) << 20)) : 0.f;
 }
-// bits: those of the value without its sign; top: the block's exponent
-__device__ __forceinline__ uint32_t encode(uint32_t bits, uint32_t r16) {
-  return min((bits + (r16 << 4)) >> 20, 2047u);  // 2047: a NaN stays one
+// r: the random bits, at the places of the value's lower mantissa. Two's complement carries
+// the difference of the exponents through the shift. NANS: a NaN's carry must not leave it.
+template <bool NANS> __device__ __forceinline__ int encode(uint32_t bits, uint32_t r, int base) {
+  if (NANS) return static_cast<int>(min((bits + r) >> 20, 2047u)) - base;
+  return static_cast<int>(bits + r - (static_cast<uint32_t>(base) << 20)) >> 20;
 }
-__device__ __forceinline__ uint32_t encode_m(float m, uint32_t r16, int top) {
-  const uint32_t b = __float_as_uint(m);
-  const int f = static_cast<int>(encode(b & 0x7fffffffu, r16)) - (8 * top - 112);
-  return f < 8 ? 0u : static_cast<uint32_t>(f) | ((b >> 24) & 128u);
+// four numbers' low bytes as one word
+__device__ __forceinline__ uint32_t word_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
-__device__ __forceinline__ uint32_t encode_v(float v, uint32_t r16, int top) {
-  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
-  const int f = static_cast<int>(encode(b, r16)) - (8 * top - 247);
-  return static_cast<uint32_t>(max(f, b ? 1 : 0));
+// The codes of four first moments: f where it is 8 or more, under the signs.
+template <bool NANS>
+__device__ __forceinline__ uint32_t encode_m4(const float* m, const uint32_t* r, int base) {
+  uint32_t b[4], f[4];
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    b[h] = __float_as_uint(m[h]);
+    const int x = encode<NANS>(b[h] & 0x7fffffffu, (r[h] << 4) & 0xffff0u, base);
+    f[h] = x < 8 ? 0u : static_cast<uint32_t>(x);
+  }
+  const uint32_t signs = __byte_perm(__byte_perm(b[0], b[1], 0x0073),
+                                     __byte_perm(b[2], b[3], 0x0073), 0x5410);
+  return word_of(f[0], f[1], f[2], f[3]) | (signs & 0x80808080u);
+}
+// The codes of four second moments (never negative): at least 1 where they are not zero.
+template <bool NANS>
+__device__ __forceinline__ uint32_t encode_v4(const float* v, const uint32_t* r, int base) {
+  uint32_t f[4];
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    const uint32_t b = __float_as_uint(v[h]);
+    f[h] = max(encode<NANS>(b, (r[h] >> 12) & 0xffff0u, base), static_cast<int>(min(b, 1u)));
+  }
+  return word_of(f[0], f[1], f[2], f[3]);
 }
 
 // Eight elements per lane, as 32 bytes of float or 16 of a 16-bit type: a warp's 256 are one
@@ -178,43 +240,45 @@ __device__ __forceinline__ void store_codes(uint8_t* p, uint2 q, bool vec, int n
   for (int k = 0; k < 8; ++k)
     if (k < n) p[k] = static_cast<uint8_t>((k < 4 ? q.x : q.y) >> (8 * (k % 4)));
 }
-__device__ __forceinline__ uint32_t code_of(uint2 q, int k) {
-  return ((k < 4 ? q.x : q.y) >> (8 * (k % 4))) & 255u;
-}
-
 // ------------------------------------------------------------------- sums of squares
 // Eight squares in float, then on in double: the norm is good to float rounding at any size.
-// Four chunks at a time, so that enough loads are in flight.
 template <typename T, int CAP>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kNormBlocks / 148)
     norm_kernel(const __grid_constant__ Table<CAP> tab, double* partials) {
-  constexpr int kAtOnce = 4;
+  constexpr int kAtOnce = sizeof(T) == 4 ? 4 : 8;
   __shared__ double part[kThreads / 32];
   double s = 0;
-  const int chunks = tab.first_chunk[tab.n];
-  for (int b0 = blockIdx.x * kAtOnce; b0 < chunks; b0 += gridDim.x * kAtOnce) {
-    float g[kAtOnce][8];
-    int k = tensor_of(tab, b0);
+  const Span span = span_of(tab);
+  int k = span.tensor;
+  auto square = [](const float (&g)[8]) {
+    float q = 0.f;
 #pragma unroll
-    for (int c = 0; c < kAtOnce; ++c) {
-      const int b = b0 + c;
+    for (int h = 0; h < 8; ++h) q = fmaf(g[h], g[h], q);
+    return q;
+  };
+  for (int b = span.at; b < span.end;) {
+    while (tab.first_chunk[k + 1] <= b) ++k;
+    const T* grad = static_cast<const T*>(tab.t[k].grad);
+    const long long n = tab.t[k].n;
+    const bool vectors = tab.vectors[k];
+    const int first = tab.first_chunk[k], stop = min(span.end, tab.first_chunk[k + 1]);
+    // whole chunks, several in flight; then what is left of the tensor or of the run
+    const int whole = vectors ? min(stop, first + static_cast<int>(n / kChunk)) : b;
+    for (; b + kAtOnce <= whole; b += kAtOnce) {
+      const T* p = grad + static_cast<long long>(b - first) * kChunk + threadIdx.x * 8;
+      float g[kAtOnce][8];
 #pragma unroll
-      for (int h = 0; h < 8; ++h) g[c][h] = 0.f;
-      if (b >= chunks) continue;
-      while (tab.first_chunk[k + 1] <= b) ++k;
-      const long long i =
-          static_cast<long long>(b - tab.first_chunk[k]) * kChunk + threadIdx.x * 8ll;
-      const long long left = static_cast<long long>(tab.t[k].n) - i;
-      if (left > 0)
-        load8(static_cast<const T*>(tab.t[k].grad) + i, g[c], tab.vectors[k] && left >= 8,
-              static_cast<int>(min(left, 8ll)));
+      for (int c = 0; c < kAtOnce; ++c) load8(p + c * kChunk, g[c]);
+#pragma unroll
+      for (int c = 0; c < kAtOnce; ++c) s += square(g[c]);
     }
-#pragma unroll
-    for (int c = 0; c < kAtOnce; ++c) {
-      float q = 0.f;
-#pragma unroll
-      for (int h = 0; h < 8; ++h) q = fmaf(g[c][h], g[c][h], q);
-      s += q;
+    for (; b < stop; ++b) {
+      const long long i = static_cast<long long>(b - first) * kChunk + threadIdx.x * 8;
+      const long long left = n - i;
+      if (left <= 0) continue;
+      float g[8];
+      load8(grad + i, g, vectors && left >= 8, static_cast<int>(min(left, 8ll)));
+      s += square(g);
     }
   }
   s = warp_sum(s);
@@ -227,68 +291,153 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // -------------------------------------------------------------------------- the step
-template <typename T, int BITS, int CAP>
-__global__ void __launch_bounds__(kThreads)
-    adamw_kernel(const __grid_constant__ Table<CAP> tab, const __grid_constant__ Opt o) {
-  const float scale = clip_scale(o);
-  const int lane = threadIdx.x & 31;
-  for (int b = blockIdx.x; b < tab.first_chunk[tab.n]; b += gridDim.x) {
-    const int k = tensor_of(tab, b);
-    const swarp_adamw_tensor_t& t = tab.t[k];
-    // the warp's block, and the lane's eight elements of it
-    const long long block = static_cast<long long>(b - tab.first_chunk[k]) * (kChunk / kBlock) +
-                            (threadIdx.x >> 5);
-    if (block * kBlock >= t.n) continue;  // the whole warp
-    const long long i = block * kBlock + lane * 8;
-    const int n = static_cast<int>(max(0ll, min(static_cast<long long>(t.n) - i, 8ll)));
-    const bool vec = tab.vectors[k] && n == 8;
-    float* pp = t.master ? t.master : static_cast<float*>(t.param);
-    float p[8], g[8];
-    load8(pp + i, p, vec, n);
-    load8(static_cast<const T*>(t.grad) + i, g, vec, n);
-    if constexpr (BITS == 32) {
-      float m[8], v[8];
-      float *pm = static_cast<float*>(t.exp_avg), *pv = static_cast<float*>(t.exp_avg_sq);
-      load8(pm + i, m, vec, n);
-      load8(pv + i, v, vec, n);
+// The new codes of a lane's eight elements from i on (a multiple of 8). NANS: the block has a
+// NaN or an infinity.
+template <bool NANS>
+__device__ __forceinline__ void encode8(const float (&m)[8], const float (&v)[8], uint32_t i,
+                                        uint32_t key, int em, int ev, uint2& cm, uint2& cv) {
+  // mix((i + h) ^ key): h is in the three lowest bits, which its first step only copies
+  const uint32_t x = i ^ key, first = x ^ (x >> 16);
+  uint32_t r[8];
 #pragma unroll
-      for (int h = 0; h < 8; ++h) {
-        const Elem e = adam(o, p[h], g[h] * scale, m[h], v[h]);
-        p[h] = e.p, m[h] = e.m, v[h] = e.v;
-      }
-      store8(pm + i, m, vec, n);
-      store8(pv + i, v, vec, n);
-    } else {
-      uint8_t *pm = static_cast<uint8_t*>(t.exp_avg), *pv = static_cast<uint8_t*>(t.exp_avg_sq);
-      const uint2 cm = load_codes(pm + i, vec, n), cv = load_codes(pv + i, vec, n);
-      const int em0 = t.exp_avg_exp[block], ev0 = t.exp_avg_sq_exp[block];
+  for (int h = 0; h < 8; ++h) r[h] = mix_on(first ^ h);
+  cm = make_uint2(encode_m4<NANS>(m, r, 8 * em - 112), encode_m4<NANS>(m + 4, r + 4, 8 * em - 112));
+  cv = make_uint2(encode_v4<NANS>(v, r, 8 * ev - 247), encode_v4<NANS>(v + 4, r + 4, 8 * ev - 247));
+}
+
+// A warp's block of one tensor, and a lane's eight elements of it
+struct Place {
+  long long block, i;
+  int n;     // elements of the lane's eight that are there
+  bool any;  // of the warp's
+  bool vec;
+  template <int CAP>
+  __device__ __forceinline__ Place(const Table<CAP>& tab, int k, int chunk) {
+    block = static_cast<long long>(chunk - tab.first_chunk[k]) * (kChunk / kBlock) +
+            (threadIdx.x >> 5);
+    i = block * kBlock + (threadIdx.x & 31) * 8;
+    const long long left = tab.t[k].n - i;
+    n = left >= 8 ? 8 : left > 0 ? static_cast<int>(left) : 0;
+    any = block * kBlock < tab.t[k].n;
+    vec = tab.vectors[k] && n == 8;
+  }
+};
+__device__ __forceinline__ float* param_of(const swarp_adamw_tensor_t& t) {
+  return t.master ? t.master : static_cast<float*>(t.param);
+}
+
+// Moments of 32 bits: one chunk per CTA. 28 bytes an element and little arithmetic; the many
+// short CTAs keep the memory busiest (150 million elements: 624 us, 104% of the copy rate,
+// against 685 with resident CTAs that walk the chunks).
+template <typename T, int CAP>
+__global__ void __launch_bounds__(kThreads, 4)
+    adamw32_kernel(const __grid_constant__ Table<CAP> tab, const __grid_constant__ Opt o) {
+  const float scale = clip_scale(o);
+  const int k = tensor_of(tab, blockIdx.x);
+  const swarp_adamw_tensor_t& t = tab.t[k];
+  const Place at(tab, k, blockIdx.x);
+  if (!at.any) return;
+  const long long i = at.i;
+  float *pp = param_of(t), *pm = static_cast<float*>(t.exp_avg),
+        *pv = static_cast<float*>(t.exp_avg_sq);
+  float p[8], g[8], m[8], v[8];
+  load8(pp + i, p, at.vec, at.n);
+  load8(static_cast<const T*>(t.grad) + i, g, at.vec, at.n);
+  load8(pm + i, m, at.vec, at.n);
+  load8(pv + i, v, at.vec, at.n);
+#pragma unroll
+  for (int h = 0; h < 8; ++h) {
+    const Elem e = adam(o, p[h], g[h] * scale, m[h], v[h]);
+    p[h] = e.p, m[h] = e.m, v[h] = e.v;
+  }
+  store8(pm + i, m, at.vec, at.n);
+  store8(pv + i, v, at.vec, at.n);
+  store8(pp + i, p, at.vec, at.n);
+  if (t.master) store8(static_cast<T*>(t.param) + i, p, at.vec, at.n);
+}
+
+// Moments of 8 bits: some 65 instructions an element against 16 bytes, so arithmetic and
+// memory take about as long. Resident CTAs walk the chunks and ask for a lane's next eight
+// elements before they work on these.
+constexpr int kResident8 = 3;
+
+template <typename T> struct Eight {
+  float p[8], g[8];
+  uint2 cm, cv;
+  int em, ev;
+  __device__ __forceinline__ void load(const swarp_adamw_tensor_t& t, const Place& at) {
+    if (!at.any) return;
+    em = t.exp_avg_exp[at.block], ev = t.exp_avg_sq_exp[at.block];
+    cm = load_codes(static_cast<const uint8_t*>(t.exp_avg) + at.i, at.vec, at.n);
+    cv = load_codes(static_cast<const uint8_t*>(t.exp_avg_sq) + at.i, at.vec, at.n);
+    load8(param_of(t) + at.i, p, at.vec, at.n);
+    load8(static_cast<const T*>(t.grad) + at.i, g, at.vec, at.n);
+  }
+};
+
+template <typename T, int CAP>
+__global__ void __launch_bounds__(kThreads, kResident8)
+    adamw8_kernel(const __grid_constant__ Table<CAP> tab, const __grid_constant__ Opt o) {
+  const float scale = clip_scale(o);
+  const int chunks = tab.first_chunk[tab.n];
+  int b = blockIdx.x, k = tensor_of(tab, b);
+  Eight<T> x, y;
+  x.load(tab.t[k], Place(tab, k, b));
+  while (true) {
+    const int b2 = b + gridDim.x;
+    int k2 = k;
+    if (b2 < chunks) {
+      while (tab.first_chunk[k2 + 1] <= b2) ++k2;
+      y.load(tab.t[k2], Place(tab, k2, b2));
+    }
+    const Place at(tab, k, b);
+    if (at.any) {
+      const swarp_adamw_tensor_t& t = tab.t[k];
+      const long long i = at.i;
       float m[8], v[8];
+      if (ordinary_exp(x.em)) {
+        const float to = __uint_as_float(static_cast<uint32_t>(x.em - 7) << 23);
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const uint32_t w = h < 2 ? x.cm.x : x.cm.y;
+          const float2 f = decode_m2(h % 2 ? w >> 16 : w & 0xffffu, to);
+          m[2 * h] = f.x, m[2 * h + 1] = f.y;
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 8; ++h) m[h] = decode_m(byte_of(h < 4 ? x.cm.x : x.cm.y, h % 4), x.em);
+      }
+      const uint32_t base = (8u * x.ev - 247u) << 20;
+#pragma unroll
+      for (int h = 0; h < 8; ++h)
+        v[h] = __uint_as_float((byte_of(h < 4 ? x.cv.x : x.cv.y, h % 4) << 20) + base);
+      if (__vcmpeq4(x.cv.x, 0) | __vcmpeq4(x.cv.y, 0)) {  // seldom: a code of zero
+#pragma unroll
+        for (int h = 0; h < 8; ++h)
+          if (byte_of(h < 4 ? x.cv.x : x.cv.y, h % 4) == 0) v[h] = 0.f;
+      }
+      // elements beyond the tensor's end are zeros, and stay zeros
       uint32_t tm = 0, tv = 0;
 #pragma unroll
       for (int h = 0; h < 8; ++h) {
-        const Elem e = adam(o, p[h], g[h] * scale, decode_m(code_of(cm, h), em0),
-                            decode_v(code_of(cv, h), ev0));
-        p[h] = e.p, m[h] = e.m, v[h] = e.v;
-        if (h < n) {
-          tm = max(tm, __float_as_uint(e.m) & 0x7fffffffu);
-          tv = max(tv, __float_as_uint(e.v) & 0x7fffffffu);
-        }
+        const Elem e = adam(o, x.p[h], x.g[h] * scale, m[h], v[h]);
+        x.p[h] = e.p, m[h] = e.m, v[h] = e.v;
+        tm = max(tm, __float_as_uint(e.m) & 0x7fffffffu);
+        tv = max(tv, __float_as_uint(e.v));
       }
+      store8(param_of(t) + i, x.p, at.vec, at.n);
+      if (t.master) store8(static_cast<T*>(t.param) + i, x.p, at.vec, at.n);
       const int em = __reduce_max_sync(kAll, tm) >> 23, ev = __reduce_max_sync(kAll, tv) >> 23;
-      uint32_t wm[2] = {0, 0}, wv[2] = {0, 0};
       const uint32_t key = tab.key[k] + static_cast<uint32_t>(i >> 32);
-#pragma unroll
-      for (int h = 0; h < 8; ++h) {
-        const uint32_t r = mix((static_cast<uint32_t>(i) + h) ^ key);
-        wm[h / 4] |= encode_m(m[h], r & 0xffffu, em) << (8 * (h % 4));
-        wv[h / 4] |= encode_v(v[h], r >> 16, ev) << (8 * (h % 4));
-      }
-      store_codes(pm + i, make_uint2(wm[0], wm[1]), vec, n);
-      store_codes(pv + i, make_uint2(wv[0], wv[1]), vec, n);
-      if (lane == 0) t.exp_avg_exp[block] = em, t.exp_avg_sq_exp[block] = ev;
+      uint2 cm, cv;
+      if (max(em, ev) < 255) encode8<false>(m, v, static_cast<uint32_t>(i), key, em, ev, cm, cv);
+      else encode8<true>(m, v, static_cast<uint32_t>(i), key, em, ev, cm, cv);
+      store_codes(static_cast<uint8_t*>(t.exp_avg) + i, cm, at.vec, at.n);
+      store_codes(static_cast<uint8_t*>(t.exp_avg_sq) + i, cv, at.vec, at.n);
+      if ((threadIdx.x & 31) == 0) t.exp_avg_exp[at.block] = em, t.exp_avg_sq_exp[at.block] = ev;
     }
-    store8(pp + i, p, vec, n);
-    if (t.master) store8(static_cast<T*>(t.param) + i, p, vec, n);
+    if (b2 >= chunks) return;
+    b = b2, k = k2, x = y;
   }
 }
 
@@ -296,16 +445,29 @@ template <typename O>
 __global__ void __launch_bounds__(kThreads)
     values_kernel(const uint8_t* codes, const uint8_t* exps, long long n, int is_signed,
                   int vectors, O* out) {
-  const long long i = (blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x) * 8;
-  if (i >= n) return;
-  const int left = static_cast<int>(min(n - i, 8ll)), e = exps[i / kBlock];
-  const bool vec = vectors && left == 8;
-  const uint2 c = load_codes(codes + i, vec, left);
-  float x[8];
+  // 16 elements per thread, in two halves
+  const long long i0 = (blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x) * 16;
+  if (i0 >= n) return;
+  const int e = exps[i0 / kBlock];
+  uint2 c[2];
+  int left[2];
+  bool vec[2];
 #pragma unroll
-  for (int h = 0; h < 8; ++h)
-    x[h] = is_signed ? decode_m(code_of(c, h), e) : decode_v(code_of(c, h), e);
-  store8(out + i, x, vec, left);
+  for (int q = 0; q < 2; ++q) {
+    left[q] = static_cast<int>(max(0ll, min(n - i0 - 8 * q, 8ll)));
+    vec[q] = vectors && left[q] == 8;
+    c[q] = load_codes(codes + i0 + 8 * q, vec[q], left[q]);
+  }
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    float x[8];
+#pragma unroll
+    for (int h = 0; h < 8; ++h) {
+      const uint32_t code = byte_of(h < 4 ? c[q].x : c[q].y, h % 4);
+      x[h] = is_signed ? decode_m(code, e) : decode_v(code, e);
+    }
+    store8(out + i0 + 8 * q, x, vec[q], left[q]);
+  }
 }
 
 // --------------------------------------------------------------------------- the host
@@ -351,11 +513,12 @@ int step_typed(const swarp_adamw_t* s, const Opt& o, const swarp_adamw_tensor_t*
   return for_each_table<CAP>(tensors, n, s->dtype, s->moment_bits, key0, s->first_tensor,
                              [&](const Table<CAP>& tab, int chunks) {
                                if (chunks == 0) return static_cast<int>(SWARP_OK);
-                               const int blocks = chunks < 148 * 8 ? chunks : 148 * 8;
+                               const int most = 148 * kResident8;
                                if (s->moment_bits == 8)
-                                 adamw_kernel<T, 8, CAP><<<blocks, kThreads, 0, st>>>(tab, o);
+                                 adamw8_kernel<T, CAP>
+                                     <<<chunks < most ? chunks : most, kThreads, 0, st>>>(tab, o);
                                else
-                                 adamw_kernel<T, 32, CAP><<<blocks, kThreads, 0, st>>>(tab, o);
+                                 adamw32_kernel<T, CAP><<<chunks, kThreads, 0, st>>>(tab, o);
                                return launch_status();
                              });
 }
@@ -448,7 +611,7 @@ int swarp_moment8_values(const uint8_t* codes, const uint8_t* exponents, int64_t
                          int32_t is_signed, int32_t dtype, void* out, void* stream) {
   if (n < 0 || (dtype != SWARP_F32 && dtype != SWARP_BF16)) return SWARP_ERR_INVALID_ARG;
   if (n == 0) return SWARP_OK;
-  const int64_t blocks = (n + 8 * kThreads - 1) / (8 * kThreads);
+  const int64_t blocks = (n + 16 * kThreads - 1) / (16 * kThreads);
   if (!codes || !exponents || !out || blocks > 0x7fffffffll) return SWARP_ERR_INVALID_ARG;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const unsigned grid = static_cast<unsigned>(blocks);

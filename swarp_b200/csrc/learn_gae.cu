@@ -28,59 +28,79 @@ __device__ __forceinline__ Step<T> load_step(const Args<T>& a, long long t, long
   s.r = a.r[k];
   s.v = a.v[k];
   s.next = a.next ? a.next[k] : T(0);
-  s.term = a.term && a.term[g];
-  // with no decay at all the next step's advantage is out, whatever it is
-  s.stop = s.term || (a.trunc && a.trunc[g]) || a.decay == T(0);
+  // both flags are asked for at once; with no decay at all the next step's advantage is out,
+  // whatever it is
+  const unsigned term = a.term ? a.term[g] : 0, trunc = a.trunc ? a.trunc[g] : 0;
+  s.term = term != 0;
+  s.stop = (term | trunc | (a.decay == T(0))) != 0;
   return s;
 }
 
 // ------------------------------------------------------------------ many columns
-// One thread per W columns (one 16-byte access, or one element) walks the steps backwards,
-// with the loads of kAhead steps in flight.
+// One thread per W columns (one 16-byte access, or one element) walks the steps backwards.
 template <typename T, int W> struct alignas(W * sizeof(T)) Pack {
   T x[W];
 };
 constexpr int kColumnThreads = 64;
 
+// kAhead steps of a thread's columns, the latest first
+template <typename T, int W, int N, bool NEXT> struct Stretch {
+  Pack<T, W> r[N], v[N], next[NEXT ? N : 1];
+  uint8_t term[N], trunc[N];
+  __device__ __forceinline__ void load(const Args<T>& a, long long t, long long j, long long f) {
+    using P = Pack<T, W>;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const long long step = t - 1 - k;
+      if (step < 0) return;
+      const long long at = step * a.columns + j, g = step * a.flags + f;
+      r[k] = *reinterpret_cast<const P*>(a.r + at);
+      v[k] = *reinterpret_cast<const P*>(a.v + at);
+      if (NEXT) next[NEXT ? k : 0] = *reinterpret_cast<const P*>(a.next + at);
+      term[k] = a.term ? a.term[g] : 0;
+      trunc[k] = a.trunc ? a.trunc[g] : 0;
+    }
+  }
+  __device__ __forceinline__ void walk(const Args<T>& a, long long t, long long j,
+                                       Pack<T, W>& A, Pack<T, W>& after) const {
+    using P = Pack<T, W>;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const long long step = t - 1 - k;
+      if (step < 0) return;
+      const bool ended = term[k], stop = term[k] | trunc[k] | (a.decay == T(0));
+      P ret;
+#pragma unroll
+      for (int c = 0; c < W; ++c) {
+        const T follow = NEXT ? next[NEXT ? k : 0].x[c] : after.x[c];
+        const T d = r[k].x[c] + (ended ? T(0) : a.gamma * follow) - v[k].x[c];
+        A.x[c] = stop ? d : d + a.decay * A.x[c];
+        ret.x[c] = A.x[c] + v[k].x[c];
+      }
+      *reinterpret_cast<P*>(a.adv + step * a.columns + j) = A;
+      *reinterpret_cast<P*>(a.ret + step * a.columns + j) = ret;
+      after = v[k];
+    }
+  }
+};
+
 template <typename T, int W, bool NEXT>
 __global__ void __launch_bounds__(kColumnThreads) gae_columns_kernel(Args<T> a) {
-  constexpr int kAhead = W == 1 ? 8 : 4;
+  constexpr int kAhead = 4;
   using P = Pack<T, W>;
   const long long j = (blockIdx.x * static_cast<long long>(kColumnThreads) + threadIdx.x) * W;
   if (j >= a.columns) return;
   const long long f = j / a.per_flag;  // W columns share their flags
   P A{}, after{};
   if (!NEXT) after = *reinterpret_cast<const P*>(a.last + j);
-  for (long long t = a.steps; t > 0; t -= kAhead) {
-    P r[kAhead], v[kAhead], next[NEXT ? kAhead : 1];
-    bool term[kAhead], stop[kAhead];
-    const int n = static_cast<int>(min(t, static_cast<long long>(kAhead)));
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if (k < n) {
-        const long long at = (t - 1 - k) * a.columns + j, g = (t - 1 - k) * a.flags + f;
-        r[k] = *reinterpret_cast<const P*>(a.r + at);
-        v[k] = *reinterpret_cast<const P*>(a.v + at);
-        if (NEXT) next[NEXT ? k : 0] = *reinterpret_cast<const P*>(a.next + at);
-        term[k] = a.term && a.term[g];
-        stop[k] = term[k] || (a.trunc && a.trunc[g]) || a.decay == T(0);
-      }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if (k < n) {
-        const long long at = (t - 1 - k) * a.columns + j;
-        P ret;
-#pragma unroll
-        for (int c = 0; c < W; ++c) {
-          const T follow = NEXT ? next[NEXT ? k : 0].x[c] : after.x[c];
-          const T d = r[k].x[c] + (term[k] ? T(0) : a.gamma * follow) - v[k].x[c];
-          A.x[c] = stop[k] ? d : d + a.decay * A.x[c];
-          ret.x[c] = A.x[c] + v[k].x[c];
-        }
-        *reinterpret_cast<P*>(a.adv + at) = A;
-        *reinterpret_cast<P*>(a.ret + at) = ret;
-        after = v[k];
-      }
+  // one stretch is on its way while the other is walked
+  Stretch<T, W, kAhead, NEXT> s0, s1;
+  s0.load(a, a.steps, j, f);
+  for (long long t = a.steps; t > 0; t -= 2 * kAhead) {
+    s1.load(a, t - kAhead, j, f);
+    s0.walk(a, t, j, A, after);
+    s0.load(a, t - 2 * kAhead, j, f);
+    s1.walk(a, t - kAhead, j, A, after);
   }
 }
 
