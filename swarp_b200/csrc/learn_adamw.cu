@@ -23,11 +23,14 @@ constexpr int kFewTensors = 24;   // launches of so few take a smaller table
 constexpr int kChunk = 2048;      // elements per CTA and turn: a block of 256 per warp
 constexpr int kNormBlocks = 592;  // partial sums of one launch
 
+// Whole chunks of the tensors whose addresses allow 16- and 32-byte accesses are numbered
+// through all tensors, and what is left of them, with the chunks of the other tensors, apart:
+// the code for the former asks nothing element by element.
 template <int CAP> struct Table {
   int n;
-  int first_chunk[CAP + 1];
+  int first_full[CAP + 1], first_part[CAP + 1];  // number of each tensor's first
   uint32_t key[CAP];
-  uint8_t vectors[CAP];  // the tensor's addresses allow 16- and 32-byte accesses
+  uint8_t vectors[CAP];
   swarp_adamw_tensor_t t[CAP];
 };
 static_assert(sizeof(Table<kMaxTensors>) < 32000, "a launch takes 32764 bytes of parameters");
@@ -58,25 +61,14 @@ __device__ __forceinline__ uint32_t mix_on(uint32_t x) {
 }
 
 // the tensor of chunk b: the last whose first chunk is not beyond it
-template <int CAP> __device__ __forceinline__ int tensor_of(const Table<CAP>& tab, int b) {
-  int lo = 0, hi = tab.n - 1;
+__device__ __forceinline__ int tensor_of(const int* first, int n, int b) {
+  int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (tab.first_chunk[mid] <= b) lo = mid;
+    if (first[mid] <= b) lo = mid;
     else hi = mid - 1;
   }
   return lo;
-}
-
-// A CTA's run of chunks, and the tensor of its first
-struct Span {
-  int at, end, tensor;
-};
-template <int CAP> __device__ __forceinline__ Span span_of(const Table<CAP>& tab) {
-  const int chunks = tab.first_chunk[tab.n];
-  const int each = (chunks + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
-  const int at = static_cast<int>(blockIdx.x) * each, end = min(at + each, chunks);
-  return Span{at, end, at < end ? tensor_of(tab, at) : 0};
 }
 
 // The gradients' scale, the same in every CTA: the partial sums added in a fixed order.
@@ -240,46 +232,81 @@ __device__ __forceinline__ void store_codes(uint8_t* p, uint2 q, bool vec, int n
   for (int k = 0; k < 8; ++k)
     if (k < n) p[k] = static_cast<uint8_t>((k < 4 ? q.x : q.y) >> (8 * (k % 4)));
 }
+// A chunk of a tensor, the same for the whole CTA, and a lane's eight elements of it: element
+// `at` of the chunk on, with the tensor's elements from `off` on. The chunk's part of an
+// address stays in uniform registers.
+struct Place {
+  long long off;
+  int room;  // the tensor's elements in the chunk
+  __device__ __forceinline__ Place(long long off, int room) : off(off), room(room) {}
+  // chunk q of those that are not whole
+  template <int CAP> __device__ __forceinline__ Place(const Table<CAP>& tab, int k, int q) {
+    const int before = tab.first_full[k + 1] - tab.first_full[k];
+    off = static_cast<long long>(q - tab.first_part[k] + before) * kChunk;
+    const long long left = tab.t[k].n - off;
+    room = left < kChunk ? static_cast<int>(left) : kChunk;
+  }
+};
+// whole chunk b
+template <int CAP>
+__device__ __forceinline__ Place whole_place(const Table<CAP>& tab, int k, int b) {
+  return Place(static_cast<long long>(b - tab.first_full[k]) * kChunk, kChunk);
+}
+struct Lane {
+  int at, n;  // the first of the lane's elements in the chunk, and how many are there
+  bool any;   // the warp has some
+  bool vec;
+  __device__ __forceinline__ Lane(const Place& p, bool vectors) {
+    at = static_cast<int>(threadIdx.x) * 8;
+    const int left = p.room - at;
+    n = left >= 8 ? 8 : left > 0 ? left : 0;
+    any = (at & ~255) < p.room;
+    vec = vectors && n == 8;
+  }
+};
+
 // ------------------------------------------------------------------- sums of squares
 // Eight squares in float, then on in double: the norm is good to float rounding at any size.
+// A CTA takes a run of whole chunks, several in flight, and its share of the others.
 template <typename T, int CAP>
 __global__ void __launch_bounds__(kThreads, kNormBlocks / 148)
     norm_kernel(const __grid_constant__ Table<CAP> tab, double* partials) {
   constexpr int kAtOnce = sizeof(T) == 4 ? 4 : 8;
   __shared__ double part[kThreads / 32];
   double s = 0;
-  const Span span = span_of(tab);
-  int k = span.tensor;
+  const int grid = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
   auto square = [](const float (&g)[8]) {
     float q = 0.f;
 #pragma unroll
     for (int h = 0; h < 8; ++h) q = fmaf(g[h], g[h], q);
     return q;
   };
-  for (int b = span.at; b < span.end;) {
-    while (tab.first_chunk[k + 1] <= b) ++k;
-    const T* grad = static_cast<const T*>(tab.t[k].grad);
-    const long long n = tab.t[k].n;
-    const bool vectors = tab.vectors[k];
-    const int first = tab.first_chunk[k], stop = min(span.end, tab.first_chunk[k + 1]);
-    // whole chunks, several in flight; then what is left of the tensor or of the run
-    const int whole = vectors ? min(stop, first + static_cast<int>(n / kChunk)) : b;
-    for (; b + kAtOnce <= whole; b += kAtOnce) {
-      const T* p = grad + static_cast<long long>(b - first) * kChunk + threadIdx.x * 8;
+  const int full = tab.first_full[tab.n], each = (full + grid - 1) / grid;
+  const int end = min((cta + 1) * each, full);
+  int b = cta * each;
+  for (int k = b < end ? tensor_of(tab.first_full, tab.n, b) : 0; b < end; ++k) {
+    const int first = tab.first_full[k], stop = min(end, tab.first_full[k + 1]);
+    const T* p = static_cast<const T*>(tab.t[k].grad) + threadIdx.x * 8;
+    for (; b + kAtOnce <= stop; b += kAtOnce) {
       float g[kAtOnce][8];
 #pragma unroll
-      for (int c = 0; c < kAtOnce; ++c) load8(p + c * kChunk, g[c]);
+      for (int c = 0; c < kAtOnce; ++c) load8(p + static_cast<long long>(b - first + c) * kChunk, g[c]);
 #pragma unroll
       for (int c = 0; c < kAtOnce; ++c) s += square(g[c]);
     }
     for (; b < stop; ++b) {
-      const long long i = static_cast<long long>(b - first) * kChunk + threadIdx.x * 8;
-      const long long left = n - i;
-      if (left <= 0) continue;
       float g[8];
-      load8(grad + i, g, vectors && left >= 8, static_cast<int>(min(left, 8ll)));
+      load8(p + static_cast<long long>(b - first) * kChunk, g);
       s += square(g);
     }
+  }
+  for (int q = cta; q < tab.first_part[tab.n]; q += grid) {
+    const int k = tensor_of(tab.first_part, tab.n, q);
+    const Place c(tab, k, q);
+    const Lane l(c, tab.vectors[k]);
+    float g[8];
+    load8(static_cast<const T*>(tab.t[k].grad) + c.off + l.at, g, l.vec, l.n);
+    s += square(g);
   }
   s = warp_sum(s);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
@@ -305,23 +332,6 @@ __device__ __forceinline__ void encode8(const float (&m)[8], const float (&v)[8]
   cv = make_uint2(encode_v4<NANS>(v, r, 8 * ev - 247), encode_v4<NANS>(v + 4, r + 4, 8 * ev - 247));
 }
 
-// A warp's block of one tensor, and a lane's eight elements of it
-struct Place {
-  long long block, i;
-  int n;     // elements of the lane's eight that are there
-  bool any;  // of the warp's
-  bool vec;
-  template <int CAP>
-  __device__ __forceinline__ Place(const Table<CAP>& tab, int k, int chunk) {
-    block = static_cast<long long>(chunk - tab.first_chunk[k]) * (kChunk / kBlock) +
-            (threadIdx.x >> 5);
-    i = block * kBlock + (threadIdx.x & 31) * 8;
-    const long long left = tab.t[k].n - i;
-    n = left >= 8 ? 8 : left > 0 ? static_cast<int>(left) : 0;
-    any = block * kBlock < tab.t[k].n;
-    vec = tab.vectors[k] && n == 8;
-  }
-};
 __device__ __forceinline__ float* param_of(const swarp_adamw_tensor_t& t) {
   return t.master ? t.master : static_cast<float*>(t.param);
 }
@@ -329,31 +339,42 @@ __device__ __forceinline__ float* param_of(const swarp_adamw_tensor_t& t) {
 // Moments of 32 bits: one chunk per CTA. 28 bytes an element and little arithmetic; the many
 // short CTAs keep the memory busiest (150 million elements: 624 us, 104% of the copy rate,
 // against 685 with resident CTAs that walk the chunks).
-template <typename T, int CAP>
-__global__ void __launch_bounds__(kThreads, 4)
-    adamw32_kernel(const __grid_constant__ Table<CAP> tab, const __grid_constant__ Opt o) {
-  const float scale = clip_scale(o);
-  const int k = tensor_of(tab, blockIdx.x);
-  const swarp_adamw_tensor_t& t = tab.t[k];
-  const Place at(tab, k, blockIdx.x);
-  if (!at.any) return;
-  const long long i = at.i;
-  float *pp = param_of(t), *pm = static_cast<float*>(t.exp_avg),
-        *pv = static_cast<float*>(t.exp_avg_sq);
+template <bool FULL, typename T>
+__device__ __forceinline__ void step32(const swarp_adamw_tensor_t& t, const Place& c,
+                                       const Lane& l, const Opt& o, float scale) {
+  float *pp = param_of(t) + c.off, *pm = static_cast<float*>(t.exp_avg) + c.off,
+        *pv = static_cast<float*>(t.exp_avg_sq) + c.off;
+  const bool vec = FULL || l.vec;
   float p[8], g[8], m[8], v[8];
-  load8(pp + i, p, at.vec, at.n);
-  load8(static_cast<const T*>(t.grad) + i, g, at.vec, at.n);
-  load8(pm + i, m, at.vec, at.n);
-  load8(pv + i, v, at.vec, at.n);
+  load8(pp + l.at, p, vec, l.n);
+  load8(static_cast<const T*>(t.grad) + c.off + l.at, g, vec, l.n);
+  load8(pm + l.at, m, vec, l.n);
+  load8(pv + l.at, v, vec, l.n);
 #pragma unroll
   for (int h = 0; h < 8; ++h) {
     const Elem e = adam(o, p[h], g[h] * scale, m[h], v[h]);
     p[h] = e.p, m[h] = e.m, v[h] = e.v;
   }
-  store8(pm + i, m, at.vec, at.n);
-  store8(pv + i, v, at.vec, at.n);
-  store8(pp + i, p, at.vec, at.n);
-  if (t.master) store8(static_cast<T*>(t.param) + i, p, at.vec, at.n);
+  store8(pm + l.at, m, vec, l.n);
+  store8(pv + l.at, v, vec, l.n);
+  store8(pp + l.at, p, vec, l.n);
+  if (t.master) store8(static_cast<T*>(t.param) + c.off + l.at, p, vec, l.n);
+}
+
+template <typename T, int CAP>
+__global__ void __launch_bounds__(kThreads, 4)
+    adamw32_kernel(const __grid_constant__ Table<CAP> tab, const __grid_constant__ Opt o) {
+  const float scale = clip_scale(o);
+  const int b = static_cast<int>(blockIdx.x), full = tab.first_full[tab.n];
+  if (b < full) {
+    const int k = tensor_of(tab.first_full, tab.n, b);
+    const Place c = whole_place(tab, k, b);
+    step32<true, T>(tab.t[k], c, Lane(c, true), o, scale);
+  } else {
+    const int k = tensor_of(tab.first_part, tab.n, b - full);
+    const Place c(tab, k, b - full);
+    step32<false, T>(tab.t[k], c, Lane(c, tab.vectors[k]), o, scale);
+  }
 }
 
 // Moments of 8 bits: some 65 instructions an element against 16 bytes, so arithmetic and
@@ -361,17 +382,73 @@ __global__ void __launch_bounds__(kThreads, 4)
 // elements before they work on these.
 constexpr int kResident8 = 3;
 
+// FULL: the chunk is whole, so no access asks.
 template <typename T> struct Eight {
   float p[8], g[8];
   uint2 cm, cv;
   int em, ev;
-  __device__ __forceinline__ void load(const swarp_adamw_tensor_t& t, const Place& at) {
-    if (!at.any) return;
-    em = t.exp_avg_exp[at.block], ev = t.exp_avg_sq_exp[at.block];
-    cm = load_codes(static_cast<const uint8_t*>(t.exp_avg) + at.i, at.vec, at.n);
-    cv = load_codes(static_cast<const uint8_t*>(t.exp_avg_sq) + at.i, at.vec, at.n);
-    load8(param_of(t) + at.i, p, at.vec, at.n);
-    load8(static_cast<const T*>(t.grad) + at.i, g, at.vec, at.n);
+
+  template <bool FULL>
+  __device__ __forceinline__ void load(const swarp_adamw_tensor_t& t, const Place& c,
+                                       const Lane& l) {
+    const long long block = c.off / kBlock;
+    em = (t.exp_avg_exp + block)[threadIdx.x >> 5];
+    ev = (t.exp_avg_sq_exp + block)[threadIdx.x >> 5];
+    cm = load_codes(static_cast<const uint8_t*>(t.exp_avg) + c.off + l.at, FULL || l.vec, l.n);
+    cv = load_codes(static_cast<const uint8_t*>(t.exp_avg_sq) + c.off + l.at, FULL || l.vec, l.n);
+    load8(param_of(t) + c.off + l.at, p, FULL || l.vec, l.n);
+    load8(static_cast<const T*>(t.grad) + c.off + l.at, g, FULL || l.vec, l.n);
+  }
+
+  template <bool FULL>
+  __device__ __forceinline__ void step(const swarp_adamw_tensor_t& t, const Place& c,
+                                       const Lane& l, const Opt& o, float scale, uint32_t key) {
+    float m[8], v[8];
+    if (ordinary_exp(em)) {
+      const float to = __uint_as_float(static_cast<uint32_t>(em - 7) << 23);
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const uint32_t w = h < 2 ? cm.x : cm.y;
+        const float2 f = decode_m2(h % 2 ? w >> 16 : w & 0xffffu, to);
+        m[2 * h] = f.x, m[2 * h + 1] = f.y;
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 8; ++h) m[h] = decode_m(byte_of(h < 4 ? cm.x : cm.y, h % 4), em);
+    }
+    const uint32_t base = (8u * ev - 247u) << 20;
+#pragma unroll
+    for (int h = 0; h < 8; ++h)
+      v[h] = __uint_as_float((byte_of(h < 4 ? cv.x : cv.y, h % 4) << 20) + base);
+    if (__vcmpeq4(cv.x, 0) | __vcmpeq4(cv.y, 0)) {  // seldom: a code of zero
+#pragma unroll
+      for (int h = 0; h < 8; ++h)
+        if (byte_of(h < 4 ? cv.x : cv.y, h % 4) == 0) v[h] = 0.f;
+    }
+    // elements beyond the tensor's end are zeros, and stay zeros
+    uint32_t tm = 0, tv = 0;
+#pragma unroll
+    for (int h = 0; h < 8; ++h) {
+      const Elem e = adam(o, p[h], g[h] * scale, m[h], v[h]);
+      p[h] = e.p, m[h] = e.m, v[h] = e.v;
+      tm = max(tm, __float_as_uint(e.m) & 0x7fffffffu);
+      tv = max(tv, __float_as_uint(e.v));
+    }
+    store8(param_of(t) + c.off + l.at, p, FULL || l.vec, l.n);
+    if (t.master) store8(static_cast<T*>(t.param) + c.off + l.at, p, FULL || l.vec, l.n);
+    const int em1 = __reduce_max_sync(kAll, tm) >> 23, ev1 = __reduce_max_sync(kAll, tv) >> 23;
+    const uint32_t i = static_cast<uint32_t>(c.off) + l.at;
+    key += static_cast<uint32_t>(c.off >> 32);
+    uint2 dm, dv;
+    if (max(em1, ev1) < 255) encode8<false>(m, v, i, key, em1, ev1, dm, dv);
+    else encode8<true>(m, v, i, key, em1, ev1, dm, dv);
+    store_codes(static_cast<uint8_t*>(t.exp_avg) + c.off + l.at, dm, FULL || l.vec, l.n);
+    store_codes(static_cast<uint8_t*>(t.exp_avg_sq) + c.off + l.at, dv, FULL || l.vec, l.n);
+    if ((threadIdx.x & 31) == 0) {
+      const long long block = c.off / kBlock;
+      (t.exp_avg_exp + block)[threadIdx.x >> 5] = static_cast<uint8_t>(em1);
+      (t.exp_avg_sq_exp + block)[threadIdx.x >> 5] = static_cast<uint8_t>(ev1);
+    }
   }
 };
 
@@ -379,65 +456,38 @@ template <typename T, int CAP>
 __global__ void __launch_bounds__(kThreads, kResident8)
     adamw8_kernel(const __grid_constant__ Table<CAP> tab, const __grid_constant__ Opt o) {
   const float scale = clip_scale(o);
-  const int chunks = tab.first_chunk[tab.n];
-  int b = blockIdx.x, k = tensor_of(tab, b);
+  const int full = tab.first_full[tab.n], parts = tab.first_part[tab.n];
+  const int by = static_cast<int>(gridDim.x);
+  for (int q = static_cast<int>(blockIdx.x); q < parts; q += by) {
+    const int k = tensor_of(tab.first_part, tab.n, q);
+    const Place c(tab, k, q);
+    const Lane l(c, tab.vectors[k]);
+    if (!l.any) continue;  // the whole warp
+    Eight<T> z;
+    z.template load<false>(tab.t[k], c, l);
+    z.template step<false>(tab.t[k], c, l, o, scale, tab.key[k]);
+  }
+  const Lane l(Place(0, kChunk), true);
+  int b = by - 1 - static_cast<int>(blockIdx.x);  // who had no part has a whole chunk first
+  if (b >= full) return;
+  int k = tensor_of(tab.first_full, tab.n, b), k2 = k;
   Eight<T> x, y;
-  x.load(tab.t[k], Place(tab, k, b));
+  x.template load<true>(tab.t[k], whole_place(tab, k, b), l);
   while (true) {
-    const int b2 = b + gridDim.x;
-    int k2 = k;
-    if (b2 < chunks) {
-      while (tab.first_chunk[k2 + 1] <= b2) ++k2;
-      y.load(tab.t[k2], Place(tab, k2, b2));
+    if (b + by < full) {
+      while (tab.first_full[k2 + 1] <= b + by) ++k2;
+      y.template load<true>(tab.t[k2], whole_place(tab, k2, b + by), l);
     }
-    const Place at(tab, k, b);
-    if (at.any) {
-      const swarp_adamw_tensor_t& t = tab.t[k];
-      const long long i = at.i;
-      float m[8], v[8];
-      if (ordinary_exp(x.em)) {
-        const float to = __uint_as_float(static_cast<uint32_t>(x.em - 7) << 23);
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const uint32_t w = h < 2 ? x.cm.x : x.cm.y;
-          const float2 f = decode_m2(h % 2 ? w >> 16 : w & 0xffffu, to);
-          m[2 * h] = f.x, m[2 * h + 1] = f.y;
-        }
-      } else {
-#pragma unroll
-        for (int h = 0; h < 8; ++h) m[h] = decode_m(byte_of(h < 4 ? x.cm.x : x.cm.y, h % 4), x.em);
-      }
-      const uint32_t base = (8u * x.ev - 247u) << 20;
-#pragma unroll
-      for (int h = 0; h < 8; ++h)
-        v[h] = __uint_as_float((byte_of(h < 4 ? x.cv.x : x.cv.y, h % 4) << 20) + base);
-      if (__vcmpeq4(x.cv.x, 0) | __vcmpeq4(x.cv.y, 0)) {  // seldom: a code of zero
-#pragma unroll
-        for (int h = 0; h < 8; ++h)
-          if (byte_of(h < 4 ? x.cv.x : x.cv.y, h % 4) == 0) v[h] = 0.f;
-      }
-      // elements beyond the tensor's end are zeros, and stay zeros
-      uint32_t tm = 0, tv = 0;
-#pragma unroll
-      for (int h = 0; h < 8; ++h) {
-        const Elem e = adam(o, x.p[h], x.g[h] * scale, m[h], v[h]);
-        x.p[h] = e.p, m[h] = e.m, v[h] = e.v;
-        tm = max(tm, __float_as_uint(e.m) & 0x7fffffffu);
-        tv = max(tv, __float_as_uint(e.v));
-      }
-      store8(param_of(t) + i, x.p, at.vec, at.n);
-      if (t.master) store8(static_cast<T*>(t.param) + i, x.p, at.vec, at.n);
-      const int em = __reduce_max_sync(kAll, tm) >> 23, ev = __reduce_max_sync(kAll, tv) >> 23;
-      const uint32_t key = tab.key[k] + static_cast<uint32_t>(i >> 32);
-      uint2 cm, cv;
-      if (max(em, ev) < 255) encode8<false>(m, v, static_cast<uint32_t>(i), key, em, ev, cm, cv);
-      else encode8<true>(m, v, static_cast<uint32_t>(i), key, em, ev, cm, cv);
-      store_codes(static_cast<uint8_t*>(t.exp_avg) + i, cm, at.vec, at.n);
-      store_codes(static_cast<uint8_t*>(t.exp_avg_sq) + i, cv, at.vec, at.n);
-      if ((threadIdx.x & 31) == 0) t.exp_avg_exp[at.block] = em, t.exp_avg_sq_exp[at.block] = ev;
+    x.template step<true>(tab.t[k], whole_place(tab, k, b), l, o, scale, tab.key[k]);
+    if ((b += by) >= full) return;
+    k = k2;
+    if (b + by < full) {
+      while (tab.first_full[k2 + 1] <= b + by) ++k2;
+      x.template load<true>(tab.t[k2], whole_place(tab, k2, b + by), l);
     }
-    if (b2 >= chunks) return;
-    b = b2, k = k2, x = y;
+    y.template step<true>(tab.t[k], whole_place(tab, k, b), l, o, scale, tab.key[k]);
+    if ((b += by) >= full) return;
+    k = k2;
   }
 }
 
@@ -489,19 +539,23 @@ int for_each_table(const swarp_adamw_tensor_t* tensors, int64_t n, int32_t dtype
   int64_t i = 0;
   do {
     tab.n = 0;
-    long long chunks = 0;
+    long long full = 0, part = 0;
     for (const int64_t end = i + CAP; i < n && i < end; ++i) {
       if (tensors[i].n == 0) continue;
-      const long long more = (tensors[i].n + kChunk - 1) / kChunk;
-      if (chunks + more > 0x3fffffffll) return SWARP_ERR_UNSUPPORTED;
+      const bool vec = vectors_ok(tensors[i], dtype, bits);
       tab.t[tab.n] = tensors[i];
-      tab.vectors[tab.n] = vectors_ok(tensors[i], dtype, bits);
+      tab.vectors[tab.n] = vec;
       tab.key[tab.n] = mix(key0 + first + static_cast<uint32_t>(i));
-      tab.first_chunk[tab.n++] = static_cast<int>(chunks);
-      chunks += more;
+      tab.first_full[tab.n] = static_cast<int>(full);
+      tab.first_part[tab.n++] = static_cast<int>(part);
+      const long long whole = vec ? tensors[i].n / kChunk : 0;
+      full += whole;
+      part += (tensors[i].n + kChunk - 1) / kChunk - whole;
+      if (full + part > 0x3fffffffll) return SWARP_ERR_UNSUPPORTED;
     }
-    tab.first_chunk[tab.n] = static_cast<int>(chunks);
-    if (const int rc = f(tab, static_cast<int>(chunks))) return rc;
+    tab.first_full[tab.n] = static_cast<int>(full);
+    tab.first_part[tab.n] = static_cast<int>(part);
+    if (const int rc = f(tab, static_cast<int>(full + part))) return rc;
   } while (i < n);
   return SWARP_OK;
 }
