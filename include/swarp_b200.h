@@ -338,7 +338,7 @@ typedef struct {
   const double* norm_partials;
   int64_t n_norm_partials;
   double max_norm;
-  float* grad_norm;     /* out: one float, the norm; or NULL */
+  float* grad_norm;     /* out: one float, the norm; required with norm_partials */
 } swarp_adamw_t;
 
 /* Number of doubles that swarp_grad_norm_partials writes for n_tensors tensors. */

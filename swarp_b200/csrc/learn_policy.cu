@@ -259,121 +259,6 @@ __global__ void __launch_bounds__(kGroupThreads) policy_group_kernel(Args a) {
   }
 }
 
-// Many short rows that lie one after the other: a CTA brings 128 of them into shared memory in
-// whole vectors, a thread takes one row from there, and the gradients go back the same way.
-// No lane waits for another's sums, and nothing is computed twice.
-constexpr int kTileRows = 128;
-
-template <typename T, int E, bool GRAD>
-__global__ void __launch_bounds__(kTileRows) policy_tile_kernel(Args a) {
-  constexpr int N = 16 / sizeof(T), kCopies = kTileRows * E / N / kTileRows;
-  __shared__ __align__(16) T tile[kTileRows * E];
-  __shared__ double part[kTileRows / 32][4];
-  const float cot = a.cotangent ? *a.cotangent : 1.f;
-  if (a.skip_unit && cot == 1.f) return;
-  const float w = row_weight(a), wg = w * a.grad_scale * cot;
-  const int V = static_cast<int>(a.vocab), tid = threadIdx.x;
-  // A row starts tid V elements in. Where that would put many threads on one bank they start
-  // at different places of their rows.
-  const int turn = sizeof(T) == 4 ? (V % 2 == 0 ? tid % V : 0) : (V % 4 == 0 ? 2 * tid % V : 0);
-  auto place = [&](int k) {
-    const int j = k + turn;
-    return tid * V + (j >= V ? j - V : j);
-  };
-  double sums[4] = {0, 0, 0, 0};
-  for (long long base = static_cast<long long>(blockIdx.x) * kTileRows; base < a.rows;
-       base += static_cast<long long>(gridDim.x) * kTileRows) {
-    const int n = static_cast<int>(min(a.rows - base, static_cast<long long>(kTileRows)));
-    const int cells = n * V, vecs = cells / N;
-    const long long i = base + tid;
-    {
-      const T* z = static_cast<const T*>(a.logits) + base * V;
-      uint4 q[kCopies];
-#pragma unroll
-      for (int k = 0; k < kCopies; ++k)
-        if (k * kTileRows + tid < vecs)
-          q[k] = *(reinterpret_cast<const uint4*>(z) + k * kTileRows + tid);
-      if (vecs * N + tid < cells) tile[vecs * N + tid] = z[vecs * N + tid];
-#pragma unroll
-      for (int k = 0; k < kCopies; ++k)
-        if (k * kTileRows + tid < vecs) reinterpret_cast<uint4*>(tile)[k * kTileRows + tid] = q[k];
-    }
-    const bool in = tid < n, live = in && (!a.mask || a.mask[i]);
-    const long long tok = live ? token_of(a, i) : 0;
-    const Inputs in0 = live ? inputs_of(a, i) : Inputs{0.f, 0.f, 0.f};
-    __syncthreads();
-    if (live) {
-      float z[E];
-      float m = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < E; ++k)
-        if (k < V) m = max_nan(m, z[k] = to_f(tile[place(k)]));
-      const float za = tok >= 0 && tok < V ? to_f(tile[tid * V + static_cast<int>(tok)]) : NAN;
-      const bool empty = m == -INFINITY;
-      if (empty) m = 0.f;
-      float s = 0.f, t = 0.f;
-#pragma unroll
-      for (int k = 0; k < E; ++k)
-        if (k < V) {
-          const float x = max_nan(z[k] - m, -1e4f);  // so that 0 x stays 0
-          z[k] = exp2_fast(x * kLog2e);
-          s += z[k];
-          t = fmaf(z[k], x, t);
-        }
-      const float ln = empty ? 0.f : __logf(s), inv = empty ? 0.f : __fdividef(1.f, s);
-      const Row r = row_terms(a, in0, empty ? (za != za ? za : -INFINITY) : (za - m) - ln,
-                              ln - t * inv, empty && za == za);
-      sums[0] += r.pg, sums[1] += r.k3, sums[2] += r.H, sums[3] += r.cut;
-      if (a.logp) a.logp[i] = r.lp, a.entropy[i] = r.H;
-      if (GRAD) {
-        const float c = wg * r.c, eta = wg * a.ent;
-        const float k0 = inv * (eta * (r.H - ln) - c), k1 = inv * eta;
-        const bool with_ent = a.ent != 0.f;
-#pragma unroll
-        for (int k = 0; k < E; ++k)
-          if (k < V) {
-            T& at = tile[place(k)];
-            float f = k0;
-            if (with_ent) f = fmaf(k1, max_nan(to_f(at) - m, -1e4f), k0);
-            at = from_f<T>(z[k] * f);
-          }
-        if (tok >= 0 && tok < V) {
-          const float x = max_nan(za - m, -1e4f);
-          tile[tid * V + static_cast<int>(tok)] =
-              from_f<T>(exp2_fast(x * kLog2e) * fmaf(k1, x, k0) + c);
-        }
-      }
-    } else if (in) {
-      if (a.logp) a.logp[i] = 0.f, a.entropy[i] = 0.f;
-      if (GRAD)
-        for (int k = 0; k < V; ++k) tile[tid * V + k] = from_f<T>(0.f);
-    }
-    __syncthreads();
-    if (GRAD) {
-      T* g = static_cast<T*>(a.grad) + base * V;
-#pragma unroll
-      for (int k = 0; k < kCopies; ++k)
-        if (k * kTileRows + tid < vecs)
-          reinterpret_cast<uint4*>(g)[k * kTileRows + tid] =
-              reinterpret_cast<const uint4*>(tile)[k * kTileRows + tid];
-      if (vecs * N + tid < cells) g[vecs * N + tid] = tile[vecs * N + tid];
-      __syncthreads();
-    }
-  }
-  if (!a.partials) return;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    sums[k] = warp_sum(sums[k]);
-    if ((tid & 31) == 0) part[tid >> 5][k] = sums[k];
-  }
-  __syncthreads();
-  if (tid < 4) {
-    double x = 0;
-    for (int q = 0; q < kTileRows / 32; ++q) x += part[q][tid];
-    a.partials[blockIdx.x * 4ll + tid] = x * w;
-  }
-}
-
 // -------------------------------------------------------------------- longer rows
 // A row is spread over a warp, a CTA or a cluster of CTAs, each thread holding NV vectors of
 // 16 bytes of it in registers, so the row is read once and its gradient written from the
@@ -808,6 +693,137 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS, 
   }
 }
 
+// ------------------------------------------------------- short rows, one after the other
+// Many short rows that lie together: a CTA brings 128 of them into shared memory in whole
+// vectors, a thread takes one row from there, and the gradients go back the same way. No lane
+// waits for another's sums, and nothing is computed twice. E - 4 < V <= E. ROT: rows of an
+// even number of words would put many threads on one bank; they then start at different
+// places of their rows.
+constexpr int kTileRows = 128;
+
+template <typename T, int E, bool ROT, bool GRAD>
+__global__ void __launch_bounds__(kTileRows, 6) policy_tile_kernel(Args a) {
+  constexpr int N = 16 / sizeof(T), kCopies = (E + N - 1) / N;
+  __shared__ __align__(16) T tile[kTileRows * E];
+  __shared__ double part[kTileRows / 32][4];
+  const float cot = a.cotangent ? *a.cotangent : 1.f;
+  if (a.skip_unit && cot == 1.f) return;
+  const int V = static_cast<int>(a.vocab), tid = threadIdx.x;
+  const int turn = ROT ? (sizeof(T) == 4 ? tid : 2 * tid) % V : 0;
+  T* mine = tile + tid * V;
+  auto place = [&](int k) -> T& {
+    int j = k;
+    if (ROT) j += turn, j = j >= V ? j - V : j;
+    return mine[j];
+  };
+  float w = 0.f, wg = 0.f;
+  float sums[4] = {0.f, 0.f, 0.f, 0.f};
+  for (long long base = static_cast<long long>(blockIdx.x) * kTileRows; base < a.rows;
+       base += static_cast<long long>(gridDim.x) * kTileRows) {
+    const int n = static_cast<int>(min(a.rows - base, static_cast<long long>(kTileRows)));
+    const int cells = n * V, vecs = cells / N;
+    const long long i = base + tid;
+    {
+      const T* z = static_cast<const T*>(a.logits) + base * V;
+      const uint4* from = reinterpret_cast<const uint4*>(z);
+#pragma unroll
+      for (int k = 0; k < kCopies; ++k)
+        if (k * kTileRows + tid < vecs)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                           shared_at(reinterpret_cast<uint4*>(tile) + k * kTileRows + tid)),
+                       "l"(from + k * kTileRows + tid)
+                       : "memory");
+      if (vecs * N + tid < cells) tile[vecs * N + tid] = z[vecs * N + tid];
+    }
+    const bool in = tid < n, live = in && (!a.mask || a.mask[i]);
+    const long long tok = live ? token_of(a, i) : 0;
+    const Inputs in0 = live ? inputs_of(a, i) : Inputs{0.f, 0.f, 0.f};
+    if (w == 0.f) w = row_weight(a), wg = w * a.grad_scale * cot;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    if (live) {
+      float x[E];
+      float m = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        x[k] = k < E - 3 || k < V ? to_f(place(k)) : -INFINITY;
+        m = max_nan(m, x[k]);
+      }
+      const bool there = tok >= 0 && tok < V;
+      const float za = there ? to_f(mine[static_cast<int>(tok)]) : NAN;
+      const bool empty = m == -INFINITY;
+      // x becomes 2^x2, the term of the sum
+      float s = 0.f, t = 0.f;
+      const float m2 = -scaled(m);
+      const bool plain = ordinary(m);
+      auto x2_of = [&](float z) {
+        return plain ? max_nan(fmaf(z, kLog2e, m2), -1e4f) : careful(z, m);
+      };
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        const float y = x2_of(x[k]);
+        x[k] = exp2_fast(y);
+        s += x[k];
+        t = fmaf(x[k], y, t);
+      }
+      const float log2s = empty ? 0.f : __log2f(s), inv = empty ? 0.f : __fdividef(1.f, s);
+      const float xa = za == -INFINITY || za != za ? za : careful(za, m) - log2s;
+      const Row r = row_terms(a, in0, xa * kLn2, (log2s - t * inv) * kLn2, empty && za == za);
+      sums[0] += r.pg, sums[1] += r.k3, sums[2] += r.H, sums[3] += r.cut;
+      if (a.logp) a.logp[i] = r.lp, a.entropy[i] = r.H;
+      if (GRAD) {
+        const float c = wg * r.c, eta = wg * a.ent;
+        const float k0 = inv * (eta * (r.H - log2s * kLn2) - c), k1 = inv * eta * kLn2;
+        float token_grad = 0.f;
+        if (there) {
+          const float y = careful(za, m);
+          token_grad = exp2_fast(y) * fmaf(k1, y, k0) + c;
+        }
+        if (a.ent == 0.f) {
+#pragma unroll
+          for (int k = 0; k < E; ++k)
+            if (k < E - 3 || k < V) place(k) = from_f<T>(x[k] * k0);
+        } else {
+#pragma unroll
+          for (int k = 0; k < E; ++k)
+            if (k < E - 3 || k < V) {
+              T& at = place(k);
+              at = from_f<T>(x[k] * fmaf(k1, x2_of(to_f(at)), k0));
+            }
+        }
+        if (there) mine[static_cast<int>(tok)] = from_f<T>(token_grad);
+      }
+    } else if (in) {
+      if (a.logp) a.logp[i] = 0.f, a.entropy[i] = 0.f;
+      if (GRAD)
+        for (int k = 0; k < V; ++k) mine[k] = from_f<T>(0.f);
+    }
+    __syncthreads();
+    if (GRAD) {
+      T* g = static_cast<T*>(a.grad) + base * V;
+#pragma unroll
+      for (int k = 0; k < kCopies; ++k)
+        if (k * kTileRows + tid < vecs)
+          reinterpret_cast<uint4*>(g)[k * kTileRows + tid] =
+              reinterpret_cast<const uint4*>(tile)[k * kTileRows + tid];
+      if (vecs * N + tid < cells) g[vecs * N + tid] = tile[vecs * N + tid];
+      __syncthreads();
+    }
+  }
+  if (!a.partials) return;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const double q = warp_sum(static_cast<double>(sums[k]));
+    if ((tid & 31) == 0) part[tid >> 5][k] = q;
+  }
+  __syncthreads();
+  if (tid < 4) {
+    double q = 0;
+    for (int k = 0; k < kTileRows / 32; ++k) q += part[k][tid];
+    a.partials[blockIdx.x * 4ll + tid] = q * w;
+  }
+}
+
 // ------------------------------------------------------------- any row, any length
 // One CTA per row at a time, the row read three times (maximum, sums, gradient), the later
 // reads from L1 or L2.
@@ -926,6 +942,7 @@ struct Plan {
 
 constexpr int kShort = 512;
 constexpr long long kManyRows = 16384;
+constexpr int kTileMaxBlocks = 148 * 32;
 
 int check(const swarp_policy_t* p) {
   if (!p || p->rows < 0 || p->vocab < 1 || p->vocab > 0x7fffffffll) return SWARP_ERR_INVALID_ARG;
@@ -944,8 +961,8 @@ Plan plan_of(const swarp_policy_t* p) {
                         reinterpret_cast<uintptr_t>(p->grad) % 16 == 0;
   if (V <= 32 && adjacent && rows >= kManyRows) {
     q.kind = kTile;
-    q.per_lane = static_cast<int>((V + 7) / 8 * 8);
-    q.blocks = q.n_partials = at_most((rows + kTileRows - 1) / kTileRows, 148 * 8);
+    q.per_lane = static_cast<int>((V + 3) / 4 * 4);
+    q.blocks = q.n_partials = at_most((rows + kTileRows - 1) / kTileRows, kTileMaxBlocks);
   } else if (V <= kShort) {
     q.kind = kGroup;
     q.lanes = V <= 4 ? 1 : V <= 8 ? 2 : V <= 16 ? 4 : V <= 32 ? 8 : V <= 64 ? 16 : 32;
@@ -977,7 +994,7 @@ Plan plan_of(const swarp_policy_t* p) {
   }
   q.partials_at = align256(kCountBlocks * sizeof(long long));
   // the same for every kind, so that it does not depend on the addresses
-  q.bytes = q.partials_at + align256(sizeof(double) * 4 * at_most(rows, kLoopMaxBlocks));
+  q.bytes = q.partials_at + align256(sizeof(double) * 4 * at_most(rows, kTileMaxBlocks));
   return q;
 }
 
@@ -991,8 +1008,10 @@ template <typename T, int L, int E, int R> int launch_group(const Args& a, const
 
 template <typename T, int E> int launch_tile(const Args& a, const Plan& q, cudaStream_t st) {
   const unsigned n = static_cast<unsigned>(q.blocks);
-  if (a.grad) policy_tile_kernel<T, E, true><<<n, kTileRows, 0, st>>>(a);
-  else policy_tile_kernel<T, E, false><<<n, kTileRows, 0, st>>>(a);
+  const bool rot = a.vocab % (sizeof(T) == 4 ? 2 : 4) == 0;
+  auto* f = a.grad ? (rot ? policy_tile_kernel<T, E, true, true> : policy_tile_kernel<T, E, false, true>)
+                   : (rot ? policy_tile_kernel<T, E, true, false> : policy_tile_kernel<T, E, false, false>);
+  f<<<n, kTileRows, 0, st>>>(a);
   return launch_status();
 }
 
@@ -1028,11 +1047,18 @@ template <typename T, int NV, int THREADS, int C> int launch_split(const Args& a
 }
 
 template <typename T> int run_typed(const Args& a, Plan& q, cudaStream_t st) {
-  if (q.kind == kTile)
-    return q.per_lane == 8    ? launch_tile<T, 8>(a, q, st)
-           : q.per_lane == 16 ? launch_tile<T, 16>(a, q, st)
-           : q.per_lane == 24 ? launch_tile<T, 24>(a, q, st)
-                              : launch_tile<T, 32>(a, q, st);
+  if (q.kind == kTile) {
+    switch (q.per_lane) {
+      case 4: return launch_tile<T, 4>(a, q, st);
+      case 8: return launch_tile<T, 8>(a, q, st);
+      case 12: return launch_tile<T, 12>(a, q, st);
+      case 16: return launch_tile<T, 16>(a, q, st);
+      case 20: return launch_tile<T, 20>(a, q, st);
+      case 24: return launch_tile<T, 24>(a, q, st);
+      case 28: return launch_tile<T, 28>(a, q, st);
+      default: return launch_tile<T, 32>(a, q, st);
+    }
+  }
   if (q.kind == kGroup) {
     switch (q.lanes) {
       case 1: return launch_group<T, 1, 4, 1>(a, q, st);
