@@ -146,25 +146,23 @@ class _PolicyLossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, batch):
         out, ctx.grad = batch.loss(True)
-        # autograd alone keeps the inputs, so that a loss kept for the record frees them
-        ctx.save_for_backward(logits, *batch.keep)
-        batch.keep = None
+        batch.out = out  # the rest of it is not differentiable and stays outside autograd
+        # autograd alone keeps the logits, so that a loss kept for the record frees them
+        rowed, *batch.keep = batch.keep
+        ctx.save_for_backward(*((logits,) if rowed is logits else (logits, rowed)))
         ctx.batch = batch
-        ctx.mark_non_differentiable(*out[1:])
-        ctx.set_materialize_grads(False)
-        return tuple(out)
+        return out.loss
 
     @staticmethod
-    def backward(ctx, g_loss, *_):
-        if g_loss is None:
-            return None, None
+    def backward(ctx, g_loss):
         if torch.is_grad_enabled():
             raise RuntimeError("policy_loss is differentiable once (create_graph is not supported)")
-        _, logits, *_ = held = ctx.saved_tensors  # noqa: F841  alive until the launch
+        logits = ctx.saved_tensors[-1]
         batch, grad, ctx.grad = ctx.batch, ctx.grad, None
         skip_unit = grad is not None
         if grad is None:  # a second backward of a retained graph: the buffer is gone
             grad = batch.new_grad(logits)
+        batch.c.logits = logits.data_ptr()
         batch.call("swarp_policy_grad", logits, g_loss.data_ptr(), int(skip_unit))
         return grad, None
 
@@ -218,7 +216,9 @@ def policy_loss(
     b = _batch(logits, tokens, old_logp, advantages, ref_logp, mask, clip_low, clip_high, kl_coef,
                entropy_coef, reduction)
     if logits.requires_grad and torch.is_grad_enabled():
-        return PolicyLoss(*_PolicyLossFn.apply(logits, b))
+        loss = _PolicyLossFn.apply(logits, b)
+        out, b.out = b.out, None
+        return out._replace(loss=loss)
     return b.loss(False)[0]
 
 
