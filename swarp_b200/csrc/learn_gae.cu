@@ -36,84 +36,8 @@ __device__ __forceinline__ Step<T> load_step(const Args<T>& a, long long t, long
   return s;
 }
 
-// ------------------------------------------------------------------ many columns
-// One thread per W columns (one 16-byte access, or one element) walks the steps backwards.
-template <typename T, int W> struct alignas(W * sizeof(T)) Pack {
-  T x[W];
-};
-constexpr int kColumnThreads = 64;
-
-// kAhead steps of a thread's columns, the latest first
-template <typename T, int W, int N, bool NEXT> struct Stretch {
-  Pack<T, W> r[N], v[N], next[NEXT ? N : 1];
-  uint8_t term[N], trunc[N];
-  __device__ __forceinline__ void load(const Args<T>& a, long long t, long long j, long long f) {
-    using P = Pack<T, W>;
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const long long step = t - 1 - k;
-      if (step < 0) return;
-      const long long at = step * a.columns + j, g = step * a.flags + f;
-      r[k] = *reinterpret_cast<const P*>(a.r + at);
-      v[k] = *reinterpret_cast<const P*>(a.v + at);
-      if (NEXT) next[NEXT ? k : 0] = *reinterpret_cast<const P*>(a.next + at);
-      term[k] = a.term ? a.term[g] : 0;
-      trunc[k] = a.trunc ? a.trunc[g] : 0;
-    }
-  }
-  __device__ __forceinline__ void walk(const Args<T>& a, long long t, long long j,
-                                       Pack<T, W>& A, Pack<T, W>& after) const {
-    using P = Pack<T, W>;
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const long long step = t - 1 - k;
-      if (step < 0) return;
-      const bool ended = term[k], stop = term[k] | trunc[k] | (a.decay == T(0));
-      P ret;
-#pragma unroll
-      for (int c = 0; c < W; ++c) {
-        const T follow = NEXT ? next[NEXT ? k : 0].x[c] : after.x[c];
-        const T d = r[k].x[c] + (ended ? T(0) : a.gamma * follow) - v[k].x[c];
-        A.x[c] = stop ? d : d + a.decay * A.x[c];
-        ret.x[c] = A.x[c] + v[k].x[c];
-      }
-      *reinterpret_cast<P*>(a.adv + step * a.columns + j) = A;
-      *reinterpret_cast<P*>(a.ret + step * a.columns + j) = ret;
-      after = v[k];
-    }
-  }
-};
-
-template <typename T, int W, bool NEXT>
-__global__ void __launch_bounds__(kColumnThreads) gae_columns_kernel(Args<T> a) {
-  constexpr int kAhead = 4;
-  using P = Pack<T, W>;
-  const long long j = (blockIdx.x * static_cast<long long>(kColumnThreads) + threadIdx.x) * W;
-  if (j >= a.columns) return;
-  const long long f = j / a.per_flag;  // W columns share their flags
-  P A{}, after{};
-  if (!NEXT) after = *reinterpret_cast<const P*>(a.last + j);
-  // one stretch is on its way while the other is walked
-  Stretch<T, W, kAhead, NEXT> s0, s1;
-  s0.load(a, a.steps, j, f);
-  for (long long t = a.steps; t > 0; t -= 2 * kAhead) {
-    s1.load(a, t - kAhead, j, f);
-    s0.walk(a, t, j, A, after);
-    s0.load(a, t - 2 * kAhead, j, f);
-    s1.walk(a, t - kAhead, j, A, after);
-  }
-}
-
-// ------------------------------------------------------------------- few columns
-// The steps are cut into segments, one per CTA, and a segment into runs of kRun steps, one
-// per thread. A run takes the advantage x after it to b + p x before it, with p the product
-// of its decays; such maps compose, so a thread forms its run's map from its own steps, the
-// CTA composes the runs', and the first kernel leaves the segment's map. The second kernel
-// composes the maps of the segments after its own, which is the advantage that follows it,
-// and walks its runs again with that.
-constexpr int kRun = 8;
-constexpr int kCtaThreads = 256;
-
+// A stretch of steps takes the advantage x after it to b + p x before it, with p the product of
+// its decays; such maps compose.
 template <typename T> struct Map {
   T p, b;  // x -> b + p x
 };
@@ -125,6 +49,125 @@ template <typename T> __device__ __forceinline__ Map<T> after(Map<T> first, Map<
 template <typename T> __device__ __forceinline__ T apply(Map<T> m, T x) {
   return m.p == T(0) ? m.b : m.b + m.p * x;
 }
+
+// ------------------------------------------------------------------ many columns
+// One thread per W columns (one 16-byte access, or one element) walks the steps backwards.
+// Where that is too few threads to keep the memory busy the steps are cut into segments: a
+// first launch leaves each segment's map, a second composes the maps of the segments after
+// its own and walks its own again.
+template <typename T, int W> struct alignas(W * sizeof(T)) Pack {
+  T x[W];
+};
+constexpr int kColumnThreads = 64;
+
+// kAhead steps of a thread's columns, the latest first
+template <typename T, int W, int N, bool NEXT> struct Stretch {
+  Pack<T, W> r[N], v[N], next[NEXT ? N : 1];
+  // one byte for all columns or, where each has its own, a byte per column; as they were
+  // loaded: an operation here would wait for each
+  uint32_t term[N], trunc[N];
+  static __device__ __forceinline__ uint32_t flags_at(const uint8_t* p, long long at, bool own) {
+    if (!p) return 0;
+    if (W == 1 || !own) return p[at];
+    return W == 2 ? *reinterpret_cast<const uint16_t*>(p + at)
+                  : *reinterpret_cast<const uint32_t*>(p + at);
+  }
+  // the steps below t, down to `low`
+  __device__ __forceinline__ void load(const Args<T>& a, long long t, long long low, long long j,
+                                       long long f) {
+    using P = Pack<T, W>;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const long long step = t - 1 - k;
+      if (step < low) return;
+      const long long at = step * a.columns + j, g = step * a.flags + f;
+      r[k] = *reinterpret_cast<const P*>(a.r + at);
+      v[k] = *reinterpret_cast<const P*>(a.v + at);
+      if (NEXT) next[NEXT ? k : 0] = *reinterpret_cast<const P*>(a.next + at);
+      term[k] = flags_at(a.term, g, a.per_flag == 1);
+      trunc[k] = flags_at(a.trunc, g, a.per_flag == 1);
+    }
+  }
+  // A: the advantages after these steps, then before them; p: the product of the decays
+  template <bool WRITE>
+  __device__ __forceinline__ void walk(const Args<T>& a, long long t, long long low, long long j,
+                                       Pack<T, W>& A, Pack<T, W>& after, Pack<T, W>& p) const {
+    using P = Pack<T, W>;
+    const int apart = a.per_flag == 1 ? 8 : 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const long long step = t - 1 - k;
+      if (step < low) return;
+      P ret;
+#pragma unroll
+      for (int c = 0; c < W; ++c) {
+        const bool ended = term[k] >> (apart * c) & 255u;
+        const bool stop = ended || (trunc[k] >> (apart * c) & 255u) || a.decay == T(0);
+        const T follow = NEXT ? next[NEXT ? k : 0].x[c] : after.x[c];
+        const T d = r[k].x[c] + (ended ? T(0) : a.gamma * follow) - v[k].x[c];
+        A.x[c] = stop ? d : d + a.decay * A.x[c];
+        ret.x[c] = A.x[c] + v[k].x[c];
+        if (!WRITE) p.x[c] = stop ? T(0) : p.x[c] * a.decay;
+      }
+      if (WRITE) {
+        *reinterpret_cast<P*>(a.adv + step * a.columns + j) = A;
+        *reinterpret_cast<P*>(a.ret + step * a.columns + j) = ret;
+      }
+      after = v[k];
+    }
+  }
+};
+
+// What the launch is of: all steps at once, the segments' maps, or the segments' steps.
+enum Part { kAllSteps, kMaps, kSteps };
+
+template <typename T, int W, bool NEXT, int PART>
+__global__ void __launch_bounds__(kColumnThreads)
+    gae_columns_kernel(Args<T> a, long long length, T* products, T* offsets) {
+  constexpr int kAhead = W == 1 && PART != kAllSteps ? 8 : 4;
+  using P = Pack<T, W>;
+  const long long thread = blockIdx.x * static_cast<long long>(kColumnThreads) + threadIdx.x;
+  const long long j = thread * W;
+  if (j >= a.columns) return;
+  const long long f = j / a.per_flag;  // the thread's first flag
+  const long long seg = PART == kAllSteps ? 0 : blockIdx.y;
+  const long long low = seg * length, high = min(a.steps, low + length);
+  P A{}, after{}, p;
+#pragma unroll
+  for (int c = 0; c < W; ++c) p.x[c] = T(1);
+  if (!NEXT)
+    after = *reinterpret_cast<const P*>(high < a.steps ? a.v + high * a.columns + j : a.last + j);
+  // one stretch is on its way while the other is walked
+  Stretch<T, W, kAhead, NEXT> s0, s1;
+  s0.load(a, high, low, j, f);
+  if (PART == kSteps) {
+    for (long long s = gridDim.y - 1; s > seg; --s) {
+      const P q = *reinterpret_cast<const P*>(products + s * a.columns + j);
+      const P b = *reinterpret_cast<const P*>(offsets + s * a.columns + j);
+#pragma unroll
+      for (int c = 0; c < W; ++c) A.x[c] = apply(Map<T>{q.x[c], b.x[c]}, A.x[c]);
+    }
+  }
+  for (long long t = high; t > low; t -= 2 * kAhead) {
+    s1.load(a, t - kAhead, low, j, f);
+    s0.template walk<PART != kMaps>(a, t, low, j, A, after, p);
+    s0.load(a, t - 2 * kAhead, low, j, f);
+    s1.template walk<PART != kMaps>(a, t - kAhead, low, j, A, after, p);
+  }
+  if (PART == kMaps) {
+    *reinterpret_cast<P*>(products + seg * a.columns + j) = p;
+    *reinterpret_cast<P*>(offsets + seg * a.columns + j) = A;
+  }
+}
+
+// ------------------------------------------------------------------- few columns
+// The steps are cut into segments, one per CTA, and a segment into runs of kRun steps, one
+// per thread. A thread forms its run's map from its own steps, the CTA composes the runs', and
+// the first kernel leaves the segment's map. The second kernel
+// composes the maps of the segments after its own, which is the advantage that follows it,
+// and walks its runs again with that.
+constexpr int kRun = 8;
+constexpr int kCtaThreads = 256;
 
 // Columns per CTA: a power of two up to 32, the least that holds them all.
 inline int tile_columns(long long columns) {
@@ -191,24 +234,53 @@ __global__ void __launch_bounds__(kCtaThreads)
   }
 }
 
-// Threads of their own for all columns keep the memory busy from about this many on.
-constexpr long long kManyColumns = 32768;
+// Below this many columns a row of them is too short to be read by threads of their own.
+constexpr long long kFewColumns = 128;
+// Threads that keep the memory busy, and the fewest steps worth a segment of their own.
+constexpr long long kEnough = 148 * 64 * 3;
+constexpr long long kShortest = 32;
 
 struct Plan {
-  bool split;
-  int tile;
-  long long segments;
-  size_t bytes;
+  bool few;
+  int tile;                       // few: columns per CTA
+  long long segments, length;     // length: steps of a segment, where not few
+  int width;                      // columns per thread, where not few
+  size_t offsets_at, bytes;
 };
 Plan plan_of(const swarp_gae_t* g) {
   Plan q{};
-  q.tile = tile_columns(g->columns);
-  q.split = g->columns < kManyColumns && g->steps > kRun;
-  if (q.split) {
+  const size_t one = g->dtype == SWARP_F32 ? sizeof(float) : sizeof(double);
+  q.few = g->columns < kFewColumns && g->steps > kRun;
+  if (q.few) {
+    q.tile = tile_columns(g->columns);
     const long long per = static_cast<long long>(kCtaThreads / q.tile) * kRun;
     q.segments = (g->steps + per - 1) / per;
-    const size_t one = g->dtype == SWARP_F32 ? sizeof(Map<float>) : sizeof(Map<double>);
-    if (q.segments > 1) q.bytes = one * q.segments * g->columns;
+    if (q.segments > 1) q.bytes = 2 * one * q.segments * g->columns;
+    return q;
+  }
+  // whole packs that share a flag or have one each, all of them aligned
+  q.width = static_cast<int>(16 / one);
+  const bool flags = g->terminated || g->truncated, own = g->columns_per_flag == 1;
+  if (g->columns % q.width != 0 || (flags && !own && g->columns_per_flag % q.width != 0))
+    q.width = 1;
+  if (own)  // a pack's flags are one access
+    for (const uint8_t* p : {g->terminated, g->truncated})
+      if (reinterpret_cast<uintptr_t>(p) % 4 != 0) q.width = 1;
+  for (const void* p : {g->rewards, g->values, g->next_values, g->last_values,
+                        static_cast<const void*>(g->advantages),
+                        static_cast<const void*>(g->returns)})
+    if (reinterpret_cast<uintptr_t>(p) % 16 != 0) q.width = 1;
+  const long long threads = g->columns / q.width;
+  long long n = threads > 0 ? (kEnough + threads - 1) / threads : 1;
+  const long long most = (g->steps + kShortest - 1) / kShortest;
+  // with more than half of them there, reading everything twice costs more than it gives
+  n = n <= 2 ? 1 : n < most ? n : most;
+  if (n < 1) n = 1;
+  q.length = (g->steps + n - 1) / n;
+  q.segments = q.length > 0 ? (g->steps + q.length - 1) / q.length : 1;
+  if (q.segments > 1) {
+    q.offsets_at = align256(one * q.segments * g->columns);
+    q.bytes = q.offsets_at + one * q.segments * g->columns;
   }
   return q;
 }
@@ -220,13 +292,33 @@ int check(const swarp_gae_t* g) {
   return SWARP_OK;
 }
 
+template <typename T, int W, bool NEXT>
+int columns(const Args<T>& a, const Plan& q, void* ws, cudaStream_t st) {
+  const long long threads = a.columns / W;
+  const dim3 grid(static_cast<unsigned>((threads + kColumnThreads - 1) / kColumnThreads),
+                  static_cast<unsigned>(q.segments));
+  if (q.segments == 1) {
+    gae_columns_kernel<T, W, NEXT, kAllSteps>
+        <<<grid, kColumnThreads, 0, st>>>(a, a.steps, nullptr, nullptr);
+    return launch_status();
+  }
+  T* products = static_cast<T*>(ws);
+  T* offsets = reinterpret_cast<T*>(static_cast<char*>(ws) + q.offsets_at);
+  gae_columns_kernel<T, W, NEXT, kMaps>
+      <<<grid, kColumnThreads, 0, st>>>(a, q.length, products, offsets);
+  if (const int rc = launch_status()) return rc;
+  gae_columns_kernel<T, W, NEXT, kSteps>
+      <<<grid, kColumnThreads, 0, st>>>(a, q.length, products, offsets);
+  return launch_status();
+}
+
 template <typename T> int run(const swarp_gae_t* g, const Plan& q, void* ws, cudaStream_t st) {
   Args<T> a{static_cast<const T*>(g->rewards), static_cast<const T*>(g->values),
             static_cast<const T*>(g->next_values), static_cast<const T*>(g->last_values),
             g->terminated, g->truncated, static_cast<T*>(g->advantages),
             static_cast<T*>(g->returns), g->steps, g->columns, g->columns / g->columns_per_flag,
             g->columns_per_flag, static_cast<T>(g->gamma), static_cast<T>(g->gamma * g->lambda)};
-  if (q.split) {
+  if (q.few) {
     Map<T>* maps = static_cast<Map<T>*>(ws);
     const long long tiles = (g->columns + q.tile - 1) / q.tile;
     const dim3 grid(static_cast<unsigned>(q.segments), static_cast<unsigned>(tiles));
@@ -237,20 +329,10 @@ template <typename T> int run(const swarp_gae_t* g, const Plan& q, void* ws, cud
     gae_segments_kernel<T, true><<<grid, kCtaThreads, 0, st>>>(a, q.tile, q.segments, maps);
     return launch_status();
   }
-  constexpr int W = 16 / sizeof(T);
-  // whole packs that share a flag, all of them aligned
-  const bool flagged = a.term || a.trunc;
-  bool packs = a.columns % W == 0 && (!flagged || a.per_flag % W == 0);
-  for (const void* p : {static_cast<const void*>(a.r), static_cast<const void*>(a.v),
-                        static_cast<const void*>(a.next), static_cast<const void*>(a.last),
-                        static_cast<const void*>(a.adv), static_cast<const void*>(a.ret)})
-    packs = packs && reinterpret_cast<uintptr_t>(p) % 16 == 0;
-  const long long threads = packs ? a.columns / W : a.columns;
-  const unsigned blocks = static_cast<unsigned>((threads + kColumnThreads - 1) / kColumnThreads);
-  auto* kernel = packs ? (a.next ? gae_columns_kernel<T, W, true> : gae_columns_kernel<T, W, false>)
-                       : (a.next ? gae_columns_kernel<T, 1, true> : gae_columns_kernel<T, 1, false>);
-  kernel<<<blocks, kColumnThreads, 0, st>>>(a);
-  return launch_status();
+  return q.width == 1 ? (a.next ? columns<T, 1, true>(a, q, ws, st)
+                                : columns<T, 1, false>(a, q, ws, st))
+                      : (a.next ? columns<T, 16 / sizeof(T), true>(a, q, ws, st)
+                                : columns<T, 16 / sizeof(T), false>(a, q, ws, st));
 }
 
 }  // namespace
