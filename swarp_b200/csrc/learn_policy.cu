@@ -280,7 +280,10 @@ __global__ void __launch_bounds__(kGroupThreads) policy_group_kernel(Args a) {
 template <typename T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int N = 4;
-  static constexpr uint32_t kNegInf = 0xff800000u;
+  static __device__ __forceinline__ uint4 all(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return make_uint4(b, b, b, b);
+  }
   static __device__ __forceinline__ float2 pair(const uint4& q, int k) {
     return k == 0 ? make_float2(__uint_as_float(q.x), __uint_as_float(q.y))
                   : make_float2(__uint_as_float(q.z), __uint_as_float(q.w));
@@ -305,7 +308,11 @@ __device__ __forceinline__ void set_word(uint4& q, int k, uint32_t v) {
 }
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
-  static constexpr uint32_t kNegInf = 0xff80ff80u;
+  static __device__ __forceinline__ uint4 all(float x) {
+    const __nv_bfloat162 h = __float2bfloat162_rn(x);
+    const uint32_t b = *reinterpret_cast<const uint32_t*>(&h);
+    return make_uint4(b, b, b, b);
+  }
   static __device__ __forceinline__ float2 pair(const uint4& q, int k) {
     const uint32_t w = word(q, k);
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
@@ -325,7 +332,11 @@ template <> struct Vec<__nv_bfloat16> {
 };
 template <> struct Vec<__half> {
   static constexpr int N = 8;
-  static constexpr uint32_t kNegInf = 0xfc00fc00u;
+  static __device__ __forceinline__ uint4 all(float x) {
+    const __half2 h = __float2half2_rn(x);
+    const uint32_t b = *reinterpret_cast<const uint32_t*>(&h);
+    return make_uint4(b, b, b, b);
+  }
   static __device__ __forceinline__ float2 pair(const uint4& q, int k) {
     const uint32_t w = word(q, k);
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
@@ -524,14 +535,13 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS, 
   auto at_token = [&](const T* z, long long tok) {
     return tok >= 0 && tok < V ? to_f(z[tok]) : NAN;
   };
-  // Whether to work on vector k. In a CTA's rows the answer is the same for a warp's lanes, and
-  // those beyond the row's end hold -inf there; a group of lanes would meet its row's end in
-  // every row, and leaves those lanes out.
-  const int asks = kLanes ? at : __shfl_sync(kAll, at, 0);
-  auto has = [&](const Cut<T>& cut, int k) { return k * kAllThreads + asks < cut.vecs; };
+  // How many vectors a warp works on in any row, the same for all its lanes. Of the last, lanes
+  // may be beyond their row's end (nowhere else: a row has V / N vectors, or one less). In a
+  // group of lanes each counts its own.
+  const int asks = kLanes ? 0 : __shfl_sync(kAll, at, 0);
+  const int of_warp = V / N > asks ? (V / N - asks + kAllThreads - 1) / kAllThreads : 0;
   auto fetch = [&](const Cut<T>& cut, int k, uint4& q) {
     const int j = k * kAllThreads + at;
-    if (!kLanes) q = make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
     if (j < cut.vecs) q = load_once(cut.vec + j);
   };
 
@@ -549,10 +559,21 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS, 
     float za = at_token(z, tok);
     bool low = false;  // the thread has met a logit of -inf: its products need care
     while (true) {
+      const int count = !kLanes            ? of_warp
+                        : cut.vecs > at ? (cut.vecs - at + kAllThreads - 1) / kAllThreads
+                                        : 0;
       Part p{max_nan(z0, z1), 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < NV; ++k)
-        if (has(cut, k)) p.m = Vec<T>::most(q[k], p.m);
+        if (kLanes ? k < count
+                   : k < count - 1 || (k == count - 1 && k * kAllThreads + at < cut.vecs))
+          p.m = Vec<T>::most(q[k], p.m);
+      // lanes beyond the row's end take a logit that adds nothing to the sums, and no NaN
+      if (!kLanes && (count - 1) * kAllThreads + at >= cut.vecs) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+          if (k == count - 1) q[k] = Vec<T>::all(p.m - 200.f - 0.25f * fabsf(p.m));
+      }
       {
         const float m = p.m, m2 = scaled(m);
         // care 0: none; 1: x2 bounded below; 2: m out of the ordinary
@@ -561,7 +582,7 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS, 
           float s[2] = {0.f, 0.f}, t[2] = {0.f, 0.f};
 #pragma unroll
           for (int k = 0; k < NV; ++k)
-            if (has(cut, k)) {
+            if (k < count) {
 #pragma unroll
               for (int h = 0; h < N / 2; ++h) {
                 float2 x = Vec<T>::pair(q[k], h);
@@ -657,7 +678,7 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS, 
           constexpr int kKind = decltype(kind)::value;
 #pragma unroll
           for (int k = 0; k < NV; ++k) {
-            if (has(cut, k)) {
+            if (k < count) {
               const int j = k * kAllThreads + at;
               uint4 out;
 #pragma unroll
