@@ -469,10 +469,12 @@ template <typename T> struct Cut {
 };
 
 constexpr int split_block(int threads) { return threads <= 32 ? 256 : threads; }
-// CTAs per SM that the registers have to allow: 24 warps of 80 registers, 16 of 128
-constexpr int split_resident(int threads, int nv) {
-  return (nv > 8 ? 512 : 768) / split_block(threads);
-}
+// Vectors that a thread holds: half of its registers, and as much of a row as makes up for
+// the row's sums and scalars, which every warp does for itself (8192 rows of 131072 bf16: 16
+// vectors 981 us, 8 with half as many threads again 1176 us).
+constexpr int NV = 16;
+// CTAs per SM that the registers have to allow: 16 warps of 128
+constexpr int split_resident(int threads) { return 512 / split_block(threads); }
 
 // THREADS of 8 to 32: a row per group of so many lanes, C = 1. Otherwise one row per cluster of
 // C CTAs of THREADS. Few lanes with many vectors each do a row's scalar part for several rows
@@ -481,8 +483,8 @@ constexpr int split_resident(int threads, int nv) {
 // its way while this one is written. The parts of a row go to all CTAs of the cluster by
 // asynchronous stores that a barrier in the receiver's shared memory counts: a cluster
 // barrier would first wait for the gradient's stores.
-template <typename T, int NV, int THREADS, int C, bool GRAD>
-__global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS, NV))
+template <typename T, int THREADS, int C, bool GRAD>
+__global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS))
     policy_split_kernel(Args a) {
   constexpr bool kLanes = THREADS <= 32;
   constexpr int G = kLanes ? THREADS : 32;  // lanes that join by shuffles
@@ -1002,7 +1004,7 @@ enum Kind { kTile, kGroup, kLaneRows, kSplit, kLoop };
 struct Plan {
   Kind kind;
   int lanes, per_lane, rows_each;  // kGroup: L, E, R; kTile: per_lane = E
-  int nv, threads, cluster;        // kLaneRows, kSplit
+  int threads, cluster;            // kLaneRows, kSplit
   long long blocks, n_partials;
   size_t partials_at, bytes;
 };
@@ -1043,21 +1045,22 @@ Plan plan_of(const swarp_policy_t* p) {
     const long long rows_per_block = kGroupThreads / q.lanes * q.rows_each;
     q.blocks = at_most((rows + rows_per_block - 1) / rows_per_block, 148 * 8);
     q.n_partials = q.blocks;
-  } else if (vecs <= 32 * 16) {
+  } else if (vecs <= 32 * NV) {
     q.kind = kLaneRows;
-    q.threads = vecs <= 8 * 16 ? 8 : vecs <= 16 * 16 ? 16 : 32;
-    q.cluster = 1, q.nv = 16;
-    const int per = 256 / q.threads;
-    q.blocks = at_most((rows + per - 1) / per, 148 * split_resident(q.threads, q.nv));
-    q.n_partials = q.blocks;
-  } else if (vecs <= 256ll * 16 * 8) {
-    q.kind = kSplit;
-    q.nv = vecs <= 256 * 4 ? 4 : vecs <= 256 * 8 ? 8 : 16;
-    q.threads = 256;
+    q.threads = vecs <= 8 * NV ? 8 : vecs <= 16 * NV ? 16 : 32;
     q.cluster = 1;
-    while (vecs > static_cast<long long>(q.cluster) * q.threads * q.nv) q.cluster *= 2;
+    const int per = 256 / q.threads;
+    q.blocks = at_most((rows + per - 1) / per, 148 * split_resident(q.threads));
+    q.n_partials = q.blocks;
+  } else if (vecs <= 8ll * 256 * NV) {
+    // no more threads than the row fills: a CTA's rows come one after the other, and smaller
+    // CTAs are more rows at once (16384 rows of 4200 bf16: 64 threads 87 us, 128 133 us)
+    q.kind = kSplit;
+    q.threads = vecs <= 64 * NV ? 64 : vecs <= 128 * NV ? 128 : 256;
+    q.cluster = 1;
+    while (vecs > static_cast<long long>(q.cluster) * q.threads * NV) q.cluster *= 2;
     // clusters; a launch may have fewer, as many as the device holds at once
-    q.n_partials = at_most(rows, 148ll * split_resident(q.threads, q.nv) / q.cluster);
+    q.n_partials = at_most(rows, 148ll * split_resident(q.threads) / q.cluster);
     q.blocks = q.n_partials * q.cluster;
   } else {
     q.kind = kLoop;
@@ -1086,10 +1089,10 @@ template <typename T, int E> int launch_tile(const Args& a, const Plan& q, cudaS
   return launch_status();
 }
 
-template <typename T, int NV, int THREADS, int C> int launch_split(const Args& a, Plan& q,
+template <typename T, int THREADS, int C> int launch_split(const Args& a, Plan& q,
                                                                    cudaStream_t st) {
-  auto* f = a.grad ? policy_split_kernel<T, NV, THREADS, C, true>
-                   : policy_split_kernel<T, NV, THREADS, C, false>;
+  auto* f = a.grad ? policy_split_kernel<T, THREADS, C, true>
+                   : policy_split_kernel<T, THREADS, C, false>;
   cudaLaunchConfig_t cfg{};
   cfg.blockDim = dim3(split_block(THREADS));
   cfg.stream = st;
@@ -1147,17 +1150,16 @@ template <typename T> int run_typed(const Args& a, Plan& q, cudaStream_t st) {
     }
   }
   if (q.kind == kLaneRows)
-    return q.threads == 8    ? launch_split<T, 16, 8, 1>(a, q, st)
-           : q.threads == 16 ? launch_split<T, 16, 16, 1>(a, q, st)
-                             : launch_split<T, 16, 32, 1>(a, q, st);
-  if (q.kind == kSplit) {
-    if (q.nv == 4) return launch_split<T, 4, 256, 1>(a, q, st);
-    if (q.nv == 8) return launch_split<T, 8, 256, 1>(a, q, st);
-    return q.cluster == 1   ? launch_split<T, 16, 256, 1>(a, q, st)
-           : q.cluster == 2 ? launch_split<T, 16, 256, 2>(a, q, st)
-           : q.cluster == 4 ? launch_split<T, 16, 256, 4>(a, q, st)
-                            : launch_split<T, 16, 256, 8>(a, q, st);
-  }
+    return q.threads == 8    ? launch_split<T, 8, 1>(a, q, st)
+           : q.threads == 16 ? launch_split<T, 16, 1>(a, q, st)
+                             : launch_split<T, 32, 1>(a, q, st);
+  if (q.kind == kSplit)
+    return q.threads == 64    ? launch_split<T, 64, 1>(a, q, st)
+           : q.threads == 128 ? launch_split<T, 128, 1>(a, q, st)
+           : q.cluster == 1   ? launch_split<T, 256, 1>(a, q, st)
+           : q.cluster == 2   ? launch_split<T, 256, 2>(a, q, st)
+           : q.cluster == 4   ? launch_split<T, 256, 4>(a, q, st)
+                              : launch_split<T, 256, 8>(a, q, st);
   const unsigned n = static_cast<unsigned>(q.blocks);
   if (a.grad) policy_loop_kernel<T, true><<<n, kLoopThreads, 0, st>>>(a);
   else policy_loop_kernel<T, false><<<n, kLoopThreads, 0, st>>>(a);
