@@ -20,7 +20,6 @@ from __future__ import annotations
 import ctypes as C
 from array import array
 from collections.abc import Sequence
-from itertools import chain
 from operator import attrgetter
 from typing import Any, NamedTuple
 
@@ -82,11 +81,12 @@ _numel, _ptr, _contiguous, _device = (torch.Tensor.numel, torch.Tensor.data_ptr,
 _dtype, _shape = attrgetter("dtype"), attrgetter("shape")
 
 
-def _same(ts, name, sizes, dtype, device):
-    """The addresses of ``ts``, once each has its parameter's size and is contiguous."""
+def _same(ts, name, sizes, dtype, device, sized=False):
+    """The addresses of ``ts``, once each has its parameter's size and is contiguous.
+    ``sized``: the sizes are known to be right."""
     if len(ts) != len(sizes):
         raise ValueError(f"{len(sizes)} params but {len(ts)} {name}")
-    if not (list(map(_numel, ts)) == sizes and set(map(_dtype, ts)) == {dtype}
+    if not ((sized or list(map(_numel, ts)) == sizes) and set(map(_dtype, ts)) == {dtype}
             and set(map(_device, ts)) == {device.index} and all(map(_contiguous, ts))):
         for i, (t, n) in enumerate(zip(ts, sizes)):
             if t.dtype != dtype or t.numel() != n or t.device != device or not t.is_contiguous():
@@ -121,10 +121,10 @@ class _Tensors:
         if self.dtype not in _PARAM_DTYPES:
             raise TypeError(f"params dtype {self.dtype}: want float32, bfloat16 or float16")
         sizes = list(map(_numel, params))
-        zero = [0] * n
-        p = _same(params, "params", sizes, self.dtype, self.device)
-        g = _same(grads, "grads", sizes, self.dtype, self.device)
-        if list(map(_shape, params)) != list(map(_shape, grads)):
+        p = _same(params, "params", sizes, self.dtype, self.device, sized=True)
+        alike = list(map(_shape, params)) == list(map(_shape, grads))
+        g = _same(grads, "grads", sizes, self.dtype, self.device, sized=alike)
+        if not alike:
             for i, (x, y) in enumerate(zip(params, grads)):
                 if x.shape != y.shape:
                     raise ValueError(f"grads[{i}] has shape {tuple(y.shape)}, its parameter "
@@ -132,7 +132,7 @@ class _Tensors:
         if self.dtype == torch.float32:
             if masters is not None:
                 raise ValueError("masters are for 16-bit parameters")
-            w = zero
+            w = None
         elif masters is None:
             raise ValueError(f"{self.dtype} parameters need float32 masters")
         else:
@@ -141,14 +141,17 @@ class _Tensors:
         if self.bits == 32:
             m = _same(exp_avg, "exp_avg", sizes, torch.float32, self.device)
             v = _same(exp_avg_sq, "exp_avg_sq", sizes, torch.float32, self.device)
-            me = ve = zero
+            me = ve = None
         else:
             blocks = [-(-x // BLOCK) for x in sizes]
             m, me = _same8(exp_avg, "exp_avg", sizes, blocks, True, self.device)
             v, ve = _same8(exp_avg_sq, "exp_avg_sq", sizes, blocks, False, self.device)
         self.params, self.keep = params, grads  # until the launch has read their addresses
         # swarp_adamw_tensor_t[n], in 64-bit words
-        self.words = array("Q", chain.from_iterable(zip(sizes, p, g, w, m, v, me, ve)))
+        self.words = array("Q", bytes(64 * n))
+        for k, column in enumerate((sizes, p, g, w, m, v, me, ve)):
+            if column is not None:
+                self.words[k::8] = array("Q", column)
         self.n, self.c = n, self.words.buffer_info()[0]
 
     def norm_partials(self, lib, out: torch.Tensor) -> None:
