@@ -301,6 +301,8 @@ typedef struct {
   void* returns;
 } swarp_gae_t;
 
+/* Bytes of device workspace of the call with this very g (its addresses count: aligned columns
+ * are taken several at a time); 0 where none is needed or g is invalid. */
 size_t swarp_gae_workspace_bytes(const swarp_gae_t* g);
 int swarp_gae(const swarp_gae_t* g, void* workspace, size_t workspace_bytes, void* stream);
 
