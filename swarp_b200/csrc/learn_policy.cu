@@ -357,20 +357,23 @@ template <> struct Vec<__half> {
   }
 };
 
-// A part of a row: the maximum m of its logits, and with x2 = (z - m) log2 e its sums of 2^x2
-// and 2^x2 x2. The exponent is one fused operation, z log2 e - m2 with m2 = log2 e m rounded
-// once: all x2 of a part are then off by the same amount, and parts are joined by the
-// difference of their m2, so the row's sums and its p = 2^x2 / S stay consistent to the last
-// bit. Where log2 e m would come near the end of the range (a row of the type's lowest value,
-// say) x2 is formed from z - m instead; between the two kinds of parts the difference is so
-// large that nothing remains of the lower.
+// A part of a row: the maximum m of its logits, and its sums of 2^x2 and 2^x2 x2. Where m is
+// ordinary, x2 is one fused operation, z log2 e - m2 with m2 = log2 e m rounded once: all x2 of
+// the part are then (z - m) log2 e plus the same rest, log2 e m - m2, and sums on one m2 stay
+// consistent to the last bit (p = 2^x2 / S). The rest is at most half an ulp of m2, so below
+// 2^-6 while |m| < 1e5; beyond, it would grow until 2^rest leaves the range, and x2 is formed
+// from z - m, without a rest. Masks that fill with a large finite number are of that kind.
 struct Part {
   float m, s, t;
 };
-__device__ __forceinline__ bool ordinary(float m) { return fabsf(m) < 1e38f; }
+__device__ __forceinline__ bool ordinary(float m) { return fabsf(m) < 1e5f; }
 __device__ __forceinline__ float origin(float m) { return m == -INFINITY ? 0.f : m; }
 // m2, rounded as such (not contracted into what it is added to)
 __device__ __forceinline__ float scaled(float m) { return __fmul_rn(m, kLog2e); }
+// what x2 is too large by (exactly)
+__device__ __forceinline__ float rest(float m) {
+  return ordinary(m) ? __fmaf_rn(m, kLog2e, -scaled(m)) : 0.f;
+}
 // x2 of z, for a part that is not ordinary or that holds -inf (2^x2 x2 is to be 0 there)
 __device__ __forceinline__ float careful(float z, float m) {
   const float x = ordinary(m) ? fmaf(z, kLog2e, -scaled(m)) : (z - origin(m)) * kLog2e;
@@ -380,10 +383,13 @@ __device__ __forceinline__ float careful(float z, float m) {
 __device__ __forceinline__ float bounded(float z, float m2) {
   return max_nan(fmaf(z, kLog2e, -m2), -1e4f);
 }
-// p with its sums on the maximum `top`, in place of its own
+// p with its sums on the maximum `top`, in place of its own; a rest is exchanged with the
+// maximum that it belongs to
 __device__ __forceinline__ void onto(Part& p, float top) {
-  const float d = max_nan(ordinary(top) ? __fsub_rn(scaled(p.m), scaled(top))
-                                        : (p.m - origin(top)) * kLog2e, -1e4f);
+  const float d = max_nan(ordinary(top) && ordinary(p.m)
+                              ? __fsub_rn(scaled(p.m), scaled(top))
+                              : (p.m - origin(top)) * kLog2e + (rest(top) - rest(p.m)),
+                          -1e4f);
   const float f = exp2_fast(d);
   p.t = fmaf(p.s, d, p.t) * f;
   p.s *= f;
@@ -712,10 +718,11 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS))
             fetch(cut2, k, q[k]);
           }
         };
-        // without the entropy term a logit of -inf needs no care
+        // without the entropy term a logit of -inf needs no care; with it, a finite one far
+        // below must not leave the range when it is multiplied by k1
         if (!ordinary(m)) write(std::integral_constant<int, 3>{});
         else if (a.ent == 0.f) write(std::integral_constant<int, 0>{});
-        else if (!low) write(std::integral_constant<int, 1>{});
+        else if (!low && fabsf(k1) < 0.5f) write(std::integral_constant<int, 1>{});
         else write(std::integral_constant<int, 2>{});
         auto alone = [&](float zj) {
           const float x = careful(zj, m);
