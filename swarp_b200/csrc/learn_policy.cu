@@ -383,6 +383,11 @@ __device__ __forceinline__ float careful(float z, float m) {
 __device__ __forceinline__ float bounded(float z, float m2) {
   return max_nan(fmaf(z, kLog2e, -m2), -1e4f);
 }
+// The log probability of logit z in a row with maximum m and log2 of its sum; however far below.
+__device__ __forceinline__ float logp_of(float z, float m, float log2s) {
+  if (m == -INFINITY) return z != z ? z : -INFINITY;  // nothing can be chosen
+  return (z - m) - (log2s - rest(m)) * kLn2;
+}
 // p with its sums on the maximum `top`, in place of its own; a rest is exchanged with the
 // maximum that it belongs to
 __device__ __forceinline__ void onto(Part& p, float top) {
@@ -671,10 +676,8 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS))
       const bool empty = p.m == -INFINITY;
       const float m = p.m, log2s = empty ? 0.f : __log2f(p.s);
       const float inv = empty ? 0.f : __fdividef(1.f, p.s);
-      // a barred token has probability 0, but one in a row of nothing else, or outside, has
-      // the logit itself
-      const float xa = za == -INFINITY || za != za ? za : careful(za, m) - log2s;
-      const Row r = row_terms(a, in, xa * kLn2, (log2s - p.t * inv) * kLn2, empty && za == za);
+      const Row r = row_terms(a, in, logp_of(za, m, log2s), (log2s - p.t * inv) * kLn2,
+                              empty && za == za);
       if (at == 0) {
         if (a.logp) a.logp[i] = r.lp, a.entropy[i] = r.H;
         sums[0] += r.pg, sums[1] += r.k3, sums[2] += r.H, sums[3] += r.cut;
@@ -840,8 +843,8 @@ __global__ void __launch_bounds__(kTileRows, 6) policy_tile_kernel(Args a) {
         t = fmaf(x[k], y, t);
       }
       const float log2s = empty ? 0.f : __log2f(s), inv = empty ? 0.f : __fdividef(1.f, s);
-      const float xa = za == -INFINITY || za != za ? za : careful(za, m) - log2s;
-      const Row r = row_terms(a, in0, xa * kLn2, (log2s - t * inv) * kLn2, empty && za == za);
+      const Row r = row_terms(a, in0, logp_of(za, m, log2s), (log2s - t * inv) * kLn2,
+                              empty && za == za);
       sums[0] += r.pg, sums[1] += r.k3, sums[2] += r.H, sums[3] += r.cut;
       if (a.logp) a.logp[i] = r.lp, a.entropy[i] = r.H;
       if (GRAD) {

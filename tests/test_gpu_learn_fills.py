@@ -128,3 +128,38 @@ def test_fills_near_the_end_of_the_range(V, dtype):
             tok[i] = V // 2
     lp = at_token(z, tok)
     compare(z, tok, (lp - 0.05).float(), adv, (lp + 0.1).float(), scale=65536.0, mean=False)
+
+
+def far_below(z, V):
+    """Tokens at 30, 1e4, 1e9, 1e30 and 3e38 below the rows' maximum, and their bound: each of
+    the two differences is rounded once."""
+    z = z.clone()
+    tok = torch.full((z.shape[0],), V - 1 - V // 5, device=DEV)
+    z[:, V // 2] = 3.0
+    z[:, V - 1 - V // 5] = torch.tensor([-30.0, -1e4, -1e9, -1e30, -3e38],
+                                        device=DEV).repeat(z.shape[0] // 5)
+    lp = at_token(z, tok)
+    return z, tok, lp, EPS * (2 * lp.abs() + V / 32 + 64)
+
+
+@pytest.mark.parametrize("V", VOCABS)
+def test_a_chosen_token_far_below(V):
+    """Its log probability has no floor, and is the same from an aligned batch and a strided one,
+    which short rows take through other kernels."""
+    z, tok, lp, tol = far_below(batch(20, V, F32, seed=V + 4)[0], V)
+    wide = torch.empty(20, V + 3, device=DEV)
+    wide[:, :V] = z
+    zero = torch.zeros(20, device=DEV)
+    for x in (z, wide[:, :V]):
+        close(swarp.token_logp(x, tok)[0], lp, tol, "logp")
+        out, grad = swarp.policy_loss_and_grad(x, tok, zero, zero + 1)
+        close(out.logp, lp, tol, "logp")
+        assert not out.loss.isnan() and not grad.isnan().any()
+
+
+@pytest.mark.parametrize("V", VOCABS)
+def test_a_barred_token_in_a_row_with_nan(V):
+    z, tok, *_ = batch(6, V, F32)
+    z[torch.arange(6), tok] = -math.inf
+    z[torch.arange(6), (tok + 1) % V] = math.nan
+    assert swarp.token_logp(z, tok)[0].isnan().all()
