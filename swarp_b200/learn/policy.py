@@ -77,8 +77,8 @@ def _rows(logits: torch.Tensor):
 
 
 class _Batch:
-    """Checked arguments as the C struct, and the tensors that it points to (``keep``, the
-    logits first)."""
+    """Checked arguments as the C struct, and the tensors that it points to (``keep``, by the
+    struct's field ``fields``, the logits first)."""
 
     def __init__(self, logits, tokens, old_logp=None, advantages=None, ref_logp=None, mask=None,
                  clip_low=0.0, clip_high=0.0, kl_coef=0.0, entropy_coef=0.0, mean=True,
@@ -93,6 +93,7 @@ class _Batch:
         rowed, rows, inner, outer_stride, inner_stride = _rows(logits)
         tokens = like(tokens, "tokens", lead, _TOKEN_DTYPES, device)
         self.keep = keep = [rowed, tokens]
+        self.fields = fields = ["logits", "tokens"]
         small = []
         for t, name, dtypes in ((old_logp, "old_logp", _F32), (advantages, "advantages", _F32),
                                 (ref_logp, "ref_logp", _F32), (mask, "mask", _BOOL)):
@@ -100,6 +101,7 @@ class _Batch:
                 constant(t, name)
                 t = like(t, name, lead, dtypes, device)
                 keep.append(t)
+                fields.append(name)
             small.append(None if t is None else t.data_ptr())
         self.c = _lib.Policy(DTYPES[logits.dtype], tokens.dtype == torch.int64, rows,
                              logits.shape[-1], inner, outer_stride, inner_stride,
@@ -111,6 +113,11 @@ class _Batch:
         entropy = torch.empty_like(logp)
         self.c.logp, self.c.entropy = logp.data_ptr(), entropy.data_ptr()
         return logp, entropy
+
+    def reads(self, tensors) -> None:
+        """Point the struct at ``tensors`` in place of ``keep``."""
+        for field, t in zip(self.fields, tensors):
+            setattr(self.c, field, t.data_ptr())
 
     def new_grad(self, logits):
         grad = (torch.empty_like(logits) if logits.is_contiguous() else
@@ -147,9 +154,14 @@ class _PolicyLossFn(torch.autograd.Function):
     def forward(ctx, logits, batch):
         out, ctx.grad = batch.loss(True)
         batch.out = out  # the rest of it is not differentiable and stays outside autograd
-        # autograd alone keeps the logits, so that a loss kept for the record frees them
-        rowed, *batch.keep = batch.keep
-        ctx.save_for_backward(*((logits,) if rowed is logits else (logits, rowed)))
+        # autograd alone keeps the inputs: a loss kept for the record frees them, and one that is
+        # written to before the backward is an error. An inference tensor cannot be kept, and
+        # has no version to compare: a copy takes its place
+        kept = [t.clone() if t.is_inference() else t for t in batch.keep]
+        if kept[0] is not logits:
+            kept.append(logits)
+        ctx.save_for_backward(*kept)
+        batch.keep = None
         ctx.batch = batch
         return out.loss
 
@@ -157,12 +169,13 @@ class _PolicyLossFn(torch.autograd.Function):
     def backward(ctx, g_loss):
         if torch.is_grad_enabled():
             raise RuntimeError("policy_loss is differentiable once (create_graph is not supported)")
-        logits = ctx.saved_tensors[-1]
+        inputs = ctx.saved_tensors
+        logits = inputs[0]
         batch, grad, ctx.grad = ctx.batch, ctx.grad, None
         skip_unit = grad is not None
         if grad is None:  # a second backward of a retained graph: the buffer is gone
             grad = batch.new_grad(logits)
-        batch.c.logits = logits.data_ptr()
+        batch.reads(inputs)
         batch.call("swarp_policy_grad", logits, g_loss.data_ptr(), int(skip_unit))
         return grad, None
 
@@ -206,7 +219,8 @@ def policy_loss(
     """The clipped policy loss, differentiable in ``logits`` (``[..., V]``, float32, bfloat16
     or float16, any strides). ``tokens`` (int64 or int32), ``old_logp``, ``advantages``,
     ``ref_logp`` (float32) and ``mask`` (bool) have the logits' leading shape and are
-    constants.
+    constants. As with any autograd operation, none of them may be written to before the
+    backward has run: that raises an error.
 
     A masked row is never read and its gradient is exactly 0, whatever its inputs hold. A
     logit of ``-inf`` is a token that cannot be chosen; a row of nothing else has ``logp``
