@@ -94,6 +94,7 @@ class _Batch:
         tokens = like(tokens, "tokens", lead, _TOKEN_DTYPES, device)
         self.keep = keep = [rowed, tokens]
         self.fields = fields = ["logits", "tokens"]
+        self.strides = rowed.stride()
         small = []
         for t, name, dtypes in ((old_logp, "old_logp", _F32), (advantages, "advantages", _F32),
                                 (ref_logp, "ref_logp", _F32), (mask, "mask", _BOOL)):
@@ -115,9 +116,17 @@ class _Batch:
         return logp, entropy
 
     def reads(self, tensors) -> None:
-        """Point the struct at ``tensors`` in place of ``keep``."""
-        for field, t in zip(self.fields, tensors):
-            setattr(self.c, field, t.data_ptr())
+        """Point the struct at ``tensors`` in place of ``keep``, with the same values: what a
+        saved-tensor hook brings back may lie in another place and in another order."""
+        keep, c = list(tensors), self.c
+        if keep[0].stride() != self.strides:
+            keep[0], _, c.inner, c.stride_outer, c.stride_inner = _rows(keep[0])
+            self.strides = keep[0].stride()
+        for k, field in enumerate(self.fields):
+            if k and not keep[k].is_contiguous():
+                keep[k] = keep[k].contiguous()
+            setattr(c, field, keep[k].data_ptr())
+        self.keep = keep
 
     def new_grad(self, logits):
         grad = (torch.empty_like(logits) if logits.is_contiguous() else
@@ -170,13 +179,13 @@ class _PolicyLossFn(torch.autograd.Function):
         if torch.is_grad_enabled():
             raise RuntimeError("policy_loss is differentiable once (create_graph is not supported)")
         inputs = ctx.saved_tensors
-        logits = inputs[0]
         batch, grad, ctx.grad = ctx.batch, ctx.grad, None
         skip_unit = grad is not None
+        batch.reads(inputs[:len(batch.fields)])
         if grad is None:  # a second backward of a retained graph: the buffer is gone
-            grad = batch.new_grad(logits)
-        batch.reads(inputs)
-        batch.call("swarp_policy_grad", logits, g_loss.data_ptr(), int(skip_unit))
+            grad = batch.new_grad(batch.keep[0])
+        batch.call("swarp_policy_grad", grad, g_loss.data_ptr(), int(skip_unit))
+        batch.keep = None
         return grad, None
 
 

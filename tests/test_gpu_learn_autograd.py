@@ -81,3 +81,27 @@ def test_inputs_that_only_the_graph_holds(scale):
     junk = [torch.full_like(v, 1) for k, v in x.items() for _ in range(4) if k != "logits"]
     (loss * scale).backward()
     assert torch.equal(leaf.grad, want) and junk
+
+
+@pytest.mark.parametrize("V", [21, 300, 5000])
+@pytest.mark.parametrize("scale", [1.0, 0.25])
+def test_inputs_that_a_hook_brings_back(scale, V):
+    """Saved tensors that wait on the host come back in other places, and a slice of a padded
+    batch comes back without the padding."""
+    B, T = 4, 10
+    x = inputs(rows=B * T, V=V)
+    want = grad_of(x, scale)
+    wide = torch.full((B, T + 2, V + 3), float("nan"), device=DEV)
+    wide[:, :T, :V] = x["logits"].view(B, T, V)
+    leaf = wide.requires_grad_(True)
+    y = {k: v.view(B, T) for k, v in x.items() if k != "logits"}
+    y["logits"] = leaf[:, :T, :V]
+    with torch.autograd.graph.save_on_cpu():
+        loss = loss_of(y).loss
+    (loss * scale).backward(retain_graph=True)
+    first, leaf.grad = leaf.grad, None
+    (loss * scale).backward()
+    for g in (first, leaf.grad):
+        # a row at another alignment may be summed in another order
+        torch.testing.assert_close(g[:, :T, :V].reshape(B * T, V), want, rtol=1e-4, atol=1e-8)
+        assert not g[:, T:].any() and not g[..., V:].any()
