@@ -7,6 +7,7 @@
 //   dloss/dz_j = c (1{j = a} - p_j) + ent p_j (ln p_j + H),        p_j = e^(z_j - m) / S
 // so one row needs its maximum, two sums, and then one more look at its logits.
 #include <atomic>
+#include <cstdlib>
 #include <type_traits>
 
 #include "learn.cuh"
@@ -18,6 +19,7 @@ namespace {
 constexpr int kCountBlocks = 64;
 constexpr int kLoopThreads = 256;
 constexpr int kLoopMaxBlocks = 148 * 8;
+constexpr long long kWaitClocks = 1ll << 31;  // about a second
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -33,6 +35,7 @@ struct Args {
   void* grad;
   long long rows, vocab, inner, stride_outer, stride_inner;
   float lo, hi, kl, ent, grad_scale;
+  long long wait_clocks;   // limit of a wait for a part of a row
   int tokens_64, mean, skip_unit, with_loss;
 };
 
@@ -437,10 +440,11 @@ __device__ __forceinline__ void mbar_expect(uint64_t* b, uint32_t bytes) {
                "r"(bytes)
                : "memory");
 }
-// whether the phase came to its end before the limit (about a second)
-__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity) {
+// Whether the phase comes to its end within some 64 tries and then `clocks` clocks of the SM; a
+// limit below zero gives it up without a look.
+__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, long long clocks) {
   const uint32_t at = shared_at(b);
-  for (int k = 0; k < (1 << 20); ++k) {
+  auto ended = [&] {
     uint32_t done;
     asm volatile(
         "{ .reg .pred p;\n"
@@ -449,8 +453,13 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity) {
         : "=r"(done)
         : "r"(at), "r"(parity)
         : "memory");
-    if (done) return true;
-  }
+    return done != 0;
+  };
+  if (clocks < 0) return false;
+  if (ended()) return true;
+  const long long from = clock64();
+  for (int k = 0; k < 64 || clock64() - from < clocks; ++k)
+    if (ended()) return true;
   return false;
 }
 // p to the same place in the shared memory of CTA `to` of the cluster, counted by its barrier
@@ -463,6 +472,13 @@ __device__ __forceinline__ void send(float4* place, uint64_t* bar, int to, Part 
       "%4}, [%5];" ::"r"(d),
       "f"(p.m), "f"(p.s), "f"(p.t), "f"(0.f), "r"(b)
       : "memory");
+}
+
+// sets a flag at the same place in the shared memory of the cluster's first CTA
+__device__ __forceinline__ void tell_first(int* flag) {
+  uint32_t d;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(d) : "r"(shared_at(flag)));
+  asm volatile("st.shared::cluster.u32 [%0], 1;" ::"r"(d) : "memory");
 }
 
 // A row as a thread of its group sees it: whole vectors, and up to N - 1 elements before them
@@ -495,7 +511,9 @@ constexpr int split_resident(int threads) { return 512 / split_block(threads); }
 // registers take the next row's vector as soon as its gradient is out, so the next row is on
 // its way while this one is written. The parts of a row go to all CTAs of the cluster by
 // asynchronous stores that a barrier in the receiver's shared memory counts: a cluster
-// barrier would first wait for the gradient's stores.
+// barrier would first wait for the gradient's stores. Each wait for parts has a limit. A warp that
+// comes to it sends no more, so all others come to theirs at the next row at the latest; what
+// they write from then on is NaN, and so is the loss.
 // 8192 rows of 131072 bf16 take 0.98 ms, 68% of the copy rate, 4096 of 32768 123 us, 68%;
 // about 18 instructions and two exponentials an element, which fill 55% of the issue slots and
 // 45% of the exponential unit, with 16 warps an SM to hide the rest.
@@ -510,6 +528,7 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS))
   constexpr int kParts = C * kWarps;
   __shared__ float4 parts[2][kLanes ? 1 : kParts];
   __shared__ uint64_t bars[2];
+  __shared__ int any_lost;  // the first CTA's is used
   const float cot = a.cotangent ? *a.cotangent : 1.f;
   if (a.skip_unit && cot == 1.f) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -520,6 +539,7 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS))
   if (C > 1) {
     if (threadIdx.x == 0) {
       mbar_init(&bars[0]), mbar_init(&bars[1]);
+      any_lost = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     cluster_sync();
@@ -532,7 +552,7 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS))
   const long long step = kLanes ? gridDim.x * static_cast<long long>(kRowsPerCta) : gridDim.x / C;
   double sums[4] = {0, 0, 0, 0};
   int turn = 0;
-  bool lost = false;  // a part did not come: all that follows is NaN
+  int lost = -1;  // the turn in which a part did not come to this warp: all that follows is NaN
 
   // the first row from i on that the mask admits; those before it get their zeros
   auto admitted = [&](long long i) {
@@ -639,15 +659,15 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS))
         if (C == 1) {
           if (lane == 0) box[warp] = make_float4(p.m, p.s, p.t, 0.f);
           __syncthreads();
-        } else {
+        } else if (lost < 0) {
           uint64_t* bar = &bars[turn & 1];
           if (threadIdx.x == 0) mbar_expect(bar, kParts * sizeof(float4));
           if (lane < C) send(&box[rank * kWarps + warp], bar, lane, p);
-          if (!lost) lost = !mbar_wait(bar, (turn >> 1) & 1);
+          if (!__all_sync(kAll, mbar_wait(bar, (turn >> 1) & 1, a.wait_clocks))) lost = turn;
         }
         constexpr int kEach = (kParts + 31) / 32;
         Part mine[kEach];
-        float top = lost ? NAN : -INFINITY;
+        float top = lost < 0 ? -INFINITY : NAN;
 #pragma unroll
         for (int k = 0; k < kEach; ++k) {
           const int j = lane + 32 * k;
@@ -748,7 +768,16 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS))
       za = at_token(z, tok);
     }
   }
-  if (C > 1) cluster_sync();  // nobody leaves while a part may still be on its way to it
+  if (C > 1) {
+    if (lost >= 0 && lane == 0) tell_first(&any_lost);
+    __syncwarp();
+    // Every warp comes here, since its waits end. After it nobody sends; parts that were waited
+    // for have come, and those that a warp gave up are given their time again, so that nobody
+    // leaves while a part may still be on its way to it.
+    cluster_sync();
+    if (lost >= 0) mbar_wait(&bars[lost & 1], (lost >> 1) & 1, kWaitClocks);
+    if (at == 0 && any_lost) sums[0] = NAN;
+  }
   if (!a.partials) return;
   if (kLanes) {
     __shared__ double part[8][4];
@@ -1184,6 +1213,13 @@ template <typename T> int run_typed(const Args& a, Plan& q, cudaStream_t st) {
   return launch_status();
 }
 
+// SWARP_POLICY_WAIT_CLOCKS (read on every call that has clusters) replaces the limit of their
+// waits; -1 lets each run out at once, for tests.
+long long wait_clocks() {
+  const char* s = std::getenv("SWARP_POLICY_WAIT_CLOCKS");
+  return s && *s ? std::atoll(s) : kWaitClocks;
+}
+
 enum Call { kLoss, kGrad, kLogp };
 
 int run(const swarp_policy_t* p, Call call, const float* cotangent, int skip_unit,
@@ -1225,6 +1261,7 @@ int run(const swarp_policy_t* p, Call call, const float* cotangent, int skip_uni
   a.mean = p->mean;
   a.skip_unit = skip_unit;
   a.with_loss = call != kLogp;
+  if (q.cluster > 1) a.wait_clocks = wait_clocks();
   if (some) {
     if (a.mask && a.mean) {
       count_kernel<<<kCountBlocks, 256, 0, st>>>(a.mask, a.rows, reinterpret_cast<long long*>(ws));
