@@ -2,7 +2,8 @@
 
 Each agent's two velocity slots are tokens: one of ``bins`` values in [-1, 1] each. An
 iteration rolls the environment out with the current policy (``Environment.step``), records
-the tokens' log probabilities (``token_logp``), estimates advantages (``gae``), and takes a
+the tokens' log probabilities (``token_logp``), estimates advantages (``gae``, with the values
+of the observations that the steps ended in, before finished environments were reset), and takes a
 few epochs of the clipped policy loss against the rollout's policy, with a divergence term
 against the iteration's first policy (``policy_loss``), stepping both networks with
 :class:`~swarp_b200.AdamW` (8-bit moments).
@@ -40,9 +41,10 @@ class TokenPolicy(torch.nn.Module):
 
 
 def rollout(env, policy, obs, steps):
-    """``steps`` steps of the environment: what the update needs, stacked ``[T, E, A, ...]``."""
+    """``steps`` steps of the environment: what the update needs, stacked ``[T, E, A, ...]``, and
+    the observation that the next rollout starts from."""
     keep: dict[str, list] = {k: [] for k in ("obs", "tokens", "logp", "rewards", "values",
-                                             "terminated", "truncated")}
+                                             "terminated", "truncated", "final")}
     with torch.no_grad():
         for _ in range(steps):
             logits, value = policy(obs)
@@ -50,12 +52,15 @@ def rollout(env, policy, obs, steps):
             logp, _ = swarp.token_logp(logits, tokens)
             actions = tokens.to(obs.dtype) * (2.0 / (policy.bins - 1)) - 1.0
             keep["obs"].append(obs)
-            obs, reward, terminated, truncated, _ = env.step(actions)
+            obs, reward, terminated, truncated, info = env.step(actions)
             for k, x in (("tokens", tokens), ("logp", logp), ("rewards", reward),
-                         ("values", value), ("terminated", terminated), ("truncated", truncated)):
+                         ("values", value), ("terminated", terminated), ("truncated", truncated),
+                         ("final", info["final_obs"])):
                 keep[k].append(x.clone())
-        last = policy(obs)[1]
-    return {k: torch.stack(v) for k, v in keep.items()}, last, obs
+        batch = {k: torch.stack(v) for k, v in keep.items()}
+        # a step's successor is what it ended in: obs belongs to the next episode after a reset
+        batch["next_values"] = policy(batch.pop("final"))[1]
+    return batch, obs
 
 
 def train(envs=1024, agents=8, steps=32, iterations=50, epochs=4, bins=21, hidden=64, lr=3e-3,
@@ -64,16 +69,18 @@ def train(envs=1024, agents=8, steps=32, iterations=50, epochs=4, bins=21, hidde
     """Train; returns the policy and the mean reward per step of each iteration."""
     torch.manual_seed(seed)
     env = swarp.make("navigation", n_envs=envs, n_agents=agents, device="cuda:0", dt=0.05,
-                     max_steps=steps, auto_reset=True, clone_outputs=True, seed=seed)
+                     max_steps=steps, auto_reset=True, clone_outputs=True, final_observation=True,
+                     seed=seed)
     obs = env.reset(seed=seed)
     policy = TokenPolicy(obs.shape[-1], bins, hidden).to(obs.device)
     optimizer = swarp.AdamW(policy.parameters(), lr=lr, weight_decay=0.0, max_norm=1.0,
                             state_bits=state_bits, seed=seed)
     rewards = []
     for it in range(iterations):
-        batch, last, obs = rollout(env, policy, obs, steps)
-        adv, returns = swarp.gae(batch["rewards"], batch["values"], last, batch["terminated"],
-                                 batch["truncated"], gamma=gamma, lam=lam)
+        batch, obs = rollout(env, policy, obs, steps)
+        adv, returns = swarp.gae(batch["rewards"], batch["values"], None, batch["terminated"],
+                                 batch["truncated"], gamma=gamma, lam=lam,
+                                 next_values=batch["next_values"])
         scaled = (adv - adv.mean()) / (adv.std() + 1e-6)
         scaled = scaled[..., None].expand_as(batch["logp"])  # both slots share it
         for _ in range(epochs):

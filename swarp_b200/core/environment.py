@@ -7,7 +7,10 @@ terminated, truncated, info)`` with the same shape (``ValueError``) and dtype
 ``auto_reset``. The physics step is the fused CUDA rollout kernel (T = 1); observation
 and reward assembly are torch ops of the scenario. ``use_graph`` and ``fused`` are
 accepted for compatibility: the step is already a single launch, and scenario
-observations run on the torch path.
+observations run on the torch path. ``final_observation`` (not in the reference) adds
+``info["final_obs"]``: what the step's own end looked like, before ``auto_reset`` put the ended
+envs into their next episodes. A truncated step's value is that observation's, not the
+returned one's.
 """
 
 from __future__ import annotations
@@ -36,6 +39,7 @@ class Environment:
         clone_outputs: bool = False,
         fused: bool | str = "auto",
         world_config: WorldConfig | None = None,
+        final_observation: bool = False,
     ) -> None:
         if n_envs < 1:
             raise ValueError(f"n_envs must be >= 1, got {n_envs}")
@@ -50,6 +54,7 @@ class Environment:
         self.max_steps = max_steps
         self.auto_reset = auto_reset
         self.clone_outputs = clone_outputs
+        self.final_observation = final_observation
         self.world = scenario.make_world(n_envs=n_envs, device=self.device, dt=dt,
                                          substeps=substeps, dtype=dtype, world_config=world_config)
         self.n_agents = self.world.n_agents
@@ -110,6 +115,8 @@ class Environment:
         else:
             truncated = self._never_truncated
         info: dict[str, Any] = self.scenario.info()
+        if self.final_observation:
+            info["final_obs"] = self.scenario.observations()
         if self.auto_reset:
             ended = terminated | truncated
             with torch.no_grad():

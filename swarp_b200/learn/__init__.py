@@ -1,6 +1,7 @@
 """Policy training on the simulator's rollouts: advantages, the clipped policy loss and AdamW.
 
-    advantages, returns = gae(rewards, values, last_values, terminated, truncated)
+    advantages, returns = gae(rewards, values, None, terminated, truncated,
+                              next_values=next_values)   # of info["final_obs"]
     out = policy_loss(logits, tokens, old_logp, advantages, mask=mask)
     out.loss.backward()
     optimizer.step()                                     # AdamW

@@ -4,7 +4,7 @@
     A_t     = delta_t + gamma lam A_{t+1},   returns_t = A_t + V_t
 
 with ``V'_t`` dropped at a terminated step and ``A_{t+1}`` at a terminated or truncated one:
-what ``Environment.step`` returns over T steps, in one launch (two for a long rollout of few
+what ``Environment.step`` returns over T steps (``V'_t`` is the value of ``info["final_obs"]``), in one launch (two for a long rollout of few
 columns, which is split along time). The reference's trainer loops over the steps in torch.
 """
 
@@ -50,7 +50,8 @@ def gae(
     serve ``[T, n_envs, n_agents]`` rewards. The value that follows step ``t`` is
     ``values[t + 1]``, or ``next_values[t]`` where those are given (``last_values`` may then
     be ``None``): give them when episodes are truncated and reset inside the rollout, where
-    ``values[t + 1]`` already belongs to the next episode. A value that a terminated step
+    ``values[t + 1]`` already belongs to the next episode; ``Environment(...,
+    final_observation=True)`` hands out the observations that they are of. A value that a terminated step
     drops may be anything, NaN included. The results are constants: no gradient flows.
     """
     require_cuda(rewards, "rewards")
