@@ -41,11 +41,24 @@ __device__ __forceinline__ Step<T> load_step(const Args<T>& a, long long t, long
 template <typename T> struct Map {
   T p, b;  // x -> b + p x
 };
-// an end of an episode (p = 0) keeps whatever is after it out, NaN included
-template <typename T> __device__ __forceinline__ Map<T> after(Map<T> first, Map<T> then) {
-  // `first` is the earlier stretch of time: x -> first(then(x))
-  return Map<T>{first.p * then.p, first.p == T(0) ? first.b : first.b + first.p * then.b};
-}
+// p is 0 for an end of an episode alone, which keeps whatever is after it out, NaN included. A
+// product of decays that underflows stays at the least number above, which still hands a NaN or
+// an infinity on and adds nothing else.
+template <typename T> __device__ __forceinline__ T least();
+template <> __device__ __forceinline__ float least<float>() { return __int_as_float(1); }
+template <> __device__ __forceinline__ double least<double>() { return __longlong_as_double(1); }
+// maps one after the other, the earliest stretch of time first: x -> first(then(x))
+template <typename T> struct Chain {
+  T p = 1, b = 0;
+  bool ended = false;
+  __device__ __forceinline__ void then(Map<T> m) {
+    const T q = p * m.p, longer = b + p * m.b;
+    b = ended ? b : longer;
+    p = q == T(0) ? least<T>() : q;
+    ended |= m.p == T(0);
+  }
+  __device__ __forceinline__ Map<T> map() const { return Map<T>{ended ? T(0) : p, b}; }
+};
 template <typename T> __device__ __forceinline__ T apply(Map<T> m, T x) {
   return m.p == T(0) ? m.b : m.b + m.p * x;
 }
@@ -111,7 +124,8 @@ template <typename T, int W, int N, bool NEXT> struct Stretch {
         const T d = r[k].x[c] + (ended ? T(0) : a.gamma * follow) - v[k].x[c];
         A.x[c] = stop ? d : d + a.decay * A.x[c];
         ret.x[c] = A.x[c] + v[k].x[c];
-        if (!WRITE) p.x[c] = stop ? T(0) : p.x[c] * a.decay;
+        // an end is -0, and stays -0, which tells it from an underflow
+        if (!WRITE) p.x[c] = stop ? -T(0) : p.x[c] * a.decay;
       }
       if (WRITE) {
         *reinterpret_cast<P*>(a.adv + step * a.columns + j) = A;
@@ -159,6 +173,9 @@ __global__ void __launch_bounds__(kColumnThreads)
     s1.template walk<PART != kMaps>(a, t - kAhead, low, j, A, after, p);
   }
   if (PART == kMaps) {
+#pragma unroll
+    for (int c = 0; c < W; ++c)
+      if (p.x[c] == T(0) && !signbit(p.x[c]) && a.decay > T(0)) p.x[c] = least<T>();
     *reinterpret_cast<P*>(products + seg * a.columns + j) = p;
     *reinterpret_cast<P*>(offsets + seg * a.columns + j) = A;
   }
@@ -201,25 +218,29 @@ __global__ void __launch_bounds__(kCtaThreads)
   if (FINAL) {
     // the later segments in n parts, then the parts in order
     const long long later = segments - 1 - seg, each = (later + n - 1) / n;
-    Map<T> m{T(1), T(0)};
+    Chain<T> m;
     for (long long k = seg + 1 + q * each; in && k < seg + 1 + min((q + 1) * each, later); ++k)
-      m = after(m, maps[k * a.columns + j]);
-    runs[threadIdx.x] = m;
+      m.then(maps[k * a.columns + j]);
+    runs[threadIdx.x] = m.map();
     __syncthreads();
     for (int k = n - 1; k >= 0; --k) x = apply(runs[k * tile + c], x);
     __syncthreads();
   }
   T d[kRun];
   Map<T> m{T(1), T(0)};
+  bool ended = false;
 #pragma unroll
   for (int k = kRun - 1; k >= 0; --k) {
     d[k] = 0;
     if (in && t0 + k < a.steps) {
       d[k] = s[k].r + (s[k].term ? T(0) : a.gamma * (a.next ? s[k].next : after_v)) - s[k].v;
       after_v = s[k].v;
-      m = after(Map<T>{s[k].stop ? T(0) : a.decay, d[k]}, m);
+      m.b = s[k].stop ? d[k] : d[k] + a.decay * m.b;
+      m.p *= a.decay;
+      ended |= s[k].stop;
     }
   }
+  m.p = ended ? T(0) : m.p == T(0) ? least<T>() : m.p;
   runs[threadIdx.x] = m;
   __syncthreads();
   if constexpr (FINAL) {
@@ -234,8 +255,9 @@ __global__ void __launch_bounds__(kCtaThreads)
       }
     }
   } else if (q == 0 && in) {
-    for (int k = 1; k < n; ++k) m = after(m, runs[k * tile + c]);
-    maps[seg * a.columns + j] = m;
+    Chain<T> all;
+    for (int k = 0; k < n; ++k) all.then(runs[k * tile + c]);
+    maps[seg * a.columns + j] = all.map();
   }
 }
 
