@@ -29,6 +29,15 @@ from swarp_b200.learn._call import (
 
 _FLOATS = (torch.float32, torch.float64)
 _BOOL = (torch.bool,)
+_MOST_PER_FLAG = 2 ** 31 - 1  # swarp_gae_t.columns_per_flag is an int32
+
+
+def _flag_dims(shape, dims: int) -> int:
+    """Leading dimensions of ``shape`` that the flags have to have, ``dims`` at least, so that
+    the number of columns that share one fits the C struct."""
+    while math.prod(shape[dims:]) > _MOST_PER_FLAG:
+        dims += 1
+    return dims
 
 
 def gae(
@@ -86,7 +95,13 @@ def gae(
             lead = t.shape
         flags.append(t)
     columns = math.prod(shape[1:])
-    per_flag = math.prod(shape[len(lead):]) if lead is not None else 1
+    per_flag = 1
+    if lead is not None:
+        dims = _flag_dims(shape, len(lead))
+        if dims > len(lead):
+            flags = [t if t is None else t.view(*lead, *[1] * (dims - len(lead)))
+                     .expand(shape[:dims]).contiguous() for t in flags]
+        per_flag = math.prod(shape[dims:])
     adv = torch.empty_like(r)
     ret = torch.empty_like(adv)
     if adv.numel() == 0:
