@@ -94,8 +94,23 @@ __device__ __forceinline__ Row row_terms(const Args& a, const Inputs& x, float l
   r.cut = cut ? 1.f : 0.f;
   r.c = cut ? 0.f : -s1;
   if (a.ref_logp) {
-    const float d = x.ref - lp, e1 = exp2_fast(d * kLog2e) - 1.f;
-    r.k3 = e1 - d;
+    const float d = x.ref - lp;
+    // e^d - d - 1 and e^d - 1 without the cancellation: d^2 (1/2 + d/6 + ... + d^7/9!), what is
+    // left out is below 2^-28 of it for |d| < 1/2. The policy is near its reference as a rule.
+    float k3 = 1.f / 362880.f;
+    k3 = fmaf(k3, d, 1.f / 40320.f);
+    k3 = fmaf(k3, d, 1.f / 5040.f);
+    k3 = fmaf(k3, d, 1.f / 720.f);
+    k3 = fmaf(k3, d, 1.f / 120.f);
+    k3 = fmaf(k3, d, 1.f / 24.f);
+    k3 = fmaf(k3, d, 1.f / 6.f);
+    k3 = fmaf(k3, d, 0.5f) * d * d;
+    float e1 = k3 + d;
+    if (!(fabsf(d) < 0.5f)) {
+      e1 = exp2_fast(d * kLog2e) - 1.f;
+      k3 = e1 - d;
+    }
+    r.k3 = k3;
     if (a.kl != 0.f) r.c -= a.kl * e1;
   }
   return r;
