@@ -171,13 +171,17 @@ class _Tensors:
         torch.autograd.graph.increment_version(self.params)
 
 
+def _check_betas(betas) -> None:
+    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+        raise ValueError(f"betas must be in [0, 1), got {betas}")
+
+
 def _check_settings(step, lr, betas, eps, weight_decay, max_norm) -> None:
     if step < 1:
         raise ValueError(f"step counts from 1, got {step}")
     if not lr >= 0.0 or not eps >= 0.0 or not weight_decay >= 0.0:
         raise ValueError(f"lr, eps and weight_decay must be >= 0, got {lr}, {eps}, {weight_decay}")
-    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
-        raise ValueError(f"betas must be in [0, 1), got {betas}")
+    _check_betas(betas)
     if max_norm is not None and not max_norm > 0.0:
         raise ValueError(f"max_norm must be > 0 (None: no clipping), got {max_norm}")
 
@@ -238,16 +242,15 @@ class AdamW(torch.optim.Optimizer):
 
     def _init_state(self, p: torch.Tensor) -> dict[str, Any]:
         st = self.state[p]
-        if not st:
-            n = p.numel()
-            st["step"] = 0
-            for name, signed in (("exp_avg", True), ("exp_avg_sq", False)):
-                if self.state_bits == 8:
-                    st[name], st[name + "_exp"] = Moment8.zeros(n, p.device, signed)[:2]
-                else:
-                    st[name] = torch.zeros(n, dtype=torch.float32, device=p.device)
-            if p.dtype != torch.float32:
-                st["master"] = p.detach().float().contiguous()
+        n = p.numel()
+        st["step"] = 0
+        for name, signed in (("exp_avg", True), ("exp_avg_sq", False)):
+            if self.state_bits == 8:
+                st[name], st[name + "_exp"] = Moment8.zeros(n, p.device, signed)[:2]
+            else:
+                st[name] = torch.zeros(n, dtype=torch.float32, device=p.device)
+        if p.dtype != torch.float32:
+            st["master"] = p.detach().float().contiguous()
         return st
 
     @torch.no_grad()
@@ -256,35 +259,18 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        # (group, dtype, device, step) -> its parameters; the index numbers all of them
-        sets: dict[tuple, list] = {}
-        index = 0
-        for gi, group in enumerate(self.param_groups):
-            for p in group["params"]:
-                if p.grad is not None:
-                    if p.grad.is_sparse:
-                        raise RuntimeError("AdamW takes dense gradients")
-                    st = self._init_state(p)
-                    st["step"] += 1
-                    sets.setdefault((gi, p.dtype, p.device, st["step"]), []).append((index, p, st))
-                index += 1
-        if not sets:
+        fresh: list[torch.Tensor] = []
+        try:
+            made, states, device = self._launches(fresh)
+        except Exception:
+            for p in fresh:  # a refused step leaves no trace
+                del self.state[p]
+            raise
+        if not made:
             return loss
         lib = library()
-        made, device = [], None
-        for (gi, dtype, dev, step), members in sets.items():
-            if device is not None and dev != device:
-                raise ValueError("AdamW steps the parameters of one device")
-            device = dev
-            # a run of consecutive indices shares a launch: the 8-bit rounding counts tensors
-            runs: list[list] = []
-            for m in members:
-                if runs and (self.state_bits == 32 or m[0] == runs[-1][-1][0] + 1):
-                    runs[-1].append(m)
-                else:
-                    runs.append([m])
-            for run in runs:
-                made.append((gi, step, run[0][0], self._tensors(run, dtype)))
+        for st in states:
+            st["step"] += 1
         partials = norm = None
         with on_device(device):
             if self.max_norm is not None:
@@ -300,11 +286,49 @@ class AdamW(torch.optim.Optimizer):
         self.grad_norm = norm
         return loss
 
+    def _launches(self, fresh):
+        """The launches of a step as ``(group, step, index of the first tensor, tensors)``, all
+        checked, the states that it steps, and its device. Parameters whose state was made
+        go to ``fresh``."""
+        # (group, dtype, device, step) -> its parameters; the index numbers all of them
+        sets: dict[tuple, list] = {}
+        index, device = 0, None
+        for gi, group in enumerate(self.param_groups):
+            _check_betas(group["betas"])
+            for p in group["params"]:
+                g = p.grad
+                if g is not None:
+                    if g.is_sparse:
+                        raise RuntimeError("AdamW takes dense gradients")
+                    dev = p.device
+                    if device is not None and dev != device:
+                        raise ValueError("AdamW steps the parameters of one device")
+                    device = dev
+                    st = self.state.get(p)
+                    if not st:
+                        fresh.append(p)
+                        st = self._init_state(p)
+                    sets.setdefault((gi, p.dtype, dev, st["step"] + 1), []).append(
+                        (index, p, g, st))
+                index += 1
+        made = []
+        for (gi, dtype, _, step), members in sets.items():
+            # a run of consecutive indices shares a launch: the 8-bit rounding counts tensors
+            runs: list[list] = []
+            for m in members:
+                if runs and (self.state_bits == 32 or m[0] == runs[-1][-1][0] + 1):
+                    runs[-1].append(m)
+                else:
+                    runs.append([m])
+            for run in runs:
+                made.append((gi, step, run[0][0], self._tensors(run, dtype)))
+        return made, [m[3] for members in sets.values() for m in members], device
+
     def _tensors(self, run, dtype) -> _Tensors:
         params, grads, m, v, w = [], [], [], [], []
-        for _, p, st in run:
+        for _, p, g, st in run:
             params.append(p)
-            grads.append(p.grad.contiguous())
+            grads.append(g.contiguous())
             if self.state_bits == 8:
                 m.append(Moment8(st["exp_avg"], st["exp_avg_exp"], True))
                 v.append(Moment8(st["exp_avg_sq"], st["exp_avg_sq_exp"], False))
