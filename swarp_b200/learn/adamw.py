@@ -109,6 +109,15 @@ def _same8(ms, name, sizes, blocks, signed, device):
             _same(exps, name + " exponents", blocks, torch.uint8, device))
 
 
+def _once(ptrs, sizes) -> None:
+    """Refuse a parameter that is there twice: one launch steps them all, and its two updates of
+    the same memory would race."""
+    seen: dict[int, int] = {}
+    for i, (x, n) in enumerate(zip(ptrs, sizes)):
+        if n and seen.setdefault(x, i) != i:
+            raise ValueError(f"params[{i}] and params[{seen[x]}] are the same memory")
+
+
 class _Tensors:
     """Checked tensors of one dtype as the C array."""
 
@@ -122,6 +131,8 @@ class _Tensors:
             raise TypeError(f"params dtype {self.dtype}: want float32, bfloat16 or float16")
         sizes = list(map(_numel, params))
         p = _same(params, "params", sizes, self.dtype, self.device, sized=True)
+        if len(set(p)) < n:
+            _once(p, sizes)
         alike = list(map(_shape, params)) == list(map(_shape, grads))
         g = _same(grads, "grads", sizes, self.dtype, self.device, sized=alike)
         if not alike:
@@ -201,7 +212,7 @@ def adamw_step(
     masters: Sequence[torch.Tensor] | None = None,
     seed: int = 0,
 ) -> torch.Tensor | None:
-    """One step in place over ``params`` (contiguous, of one dtype and device) with ``grads`` of
+    """One step in place over ``params`` (contiguous, of one dtype and device, none twice) with ``grads`` of
     the same shapes and dtype. ``exp_avg`` and ``exp_avg_sq`` are float32 tensors or
     :class:`Moment8`; 16-bit parameters need float32 ``masters``, which take the step and
     are rounded into the parameters. ``step`` counts from 1. ``seed`` is that of the random
