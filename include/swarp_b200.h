@@ -231,10 +231,10 @@ int swarp_copy_rows(void* dst, size_t dst_pitch, const void* src, size_t src_pit
  *   row loss = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
  *              + kl_coef (e^d - d - 1) - entropy_coef H
  * and the loss is its mean over the rows that mask admits (mean != 0) or its sum. A row
- * that mask leaves out is not read: its logp and entropy are 0 and its gradient is 0. A
+ * that mask leaves out adds nothing, whatever it holds: its logp, entropy and gradient are 0. A
  * logit of -inf is a token of probability 0; a row of nothing else has logp -inf, entropy 0
  * and no loss or gradient (it still counts). A token outside [0, vocab) gives NaN. With no
- * row admitted the loss is 0. */
+ * row admitted the loss is 0. A wait inside a launch that runs out gives a NaN loss too. */
 typedef struct {
   int32_t dtype;           /* of logits and grad: SWARP_F32, SWARP_BF16 or SWARP_F16 */
   int32_t tokens_64;       /* tokens are int64 (else int32) */
@@ -332,7 +332,7 @@ typedef struct {
   int32_t dtype;        /* of param and grad: SWARP_F32, SWARP_BF16 or SWARP_F16 */
   int32_t moment_bits;  /* 32 or 8 */
   int64_t step;         /* counted from 1 */
-  double lr, beta1, beta2, eps, weight_decay;
+  double lr, beta1, beta2, eps, weight_decay; /* eps below 1e-19 counts as 1e-19 */
   uint32_t seed;        /* of the 8-bit rounding */
   uint32_t first_tensor; /* index of tensors[0] in the rounding's hash */
   /* clipping: gradients are scaled by min(1, max_norm / (norm + 1e-6)) with norm the root
@@ -352,7 +352,8 @@ int swarp_grad_norm_partials(int32_t dtype, const swarp_adamw_tensor_t* tensors,
 
 /* One decoupled-weight-decay Adam step over all tensors (host array):
  *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
- *   p = p (1 - lr wd) - lr / (1 - b1^step) * m / (sqrt(v / (1 - b2^step)) + eps) */
+ *   p = p (1 - lr wd) - lr / (1 - b1^step) * m / (sqrt(v / (1 - b2^step)) + eps)
+ * No two tensors may overlap. `step` is part of the launch: a captured call repeats it. */
 int swarp_adamw_step(const swarp_adamw_t* opt, const swarp_adamw_tensor_t* tensors,
                      int64_t n_tensors, void* stream);
 

@@ -11,8 +11,11 @@ down at random so that the averages stay unbiased (to the nearest, an average th
 bytes per element instead of 28.
 
 The tensors' addresses travel in the launch's parameters: a step uploads nothing, never
-waits for the device, and can be captured in a CUDA graph (which then repeats the step
-number, and with it the bias corrections and the random bits, that it was captured with).
+waits for the device, and can be captured in a CUDA graph. The step number travels there too,
+so a graph that is replayed repeats the one that it was captured with: its bias corrections,
+which a graph captured late in training hardly notices, and with 8-bit moments the random
+bits. Each element would then always round against the same threshold, which is no longer
+unbiased: do not replay a captured 8-bit step in place of further steps.
 """
 
 from __future__ import annotations
@@ -215,7 +218,8 @@ def adamw_step(
     """One step in place over ``params`` (contiguous, of one dtype and device, none twice) with ``grads`` of
     the same shapes and dtype. ``exp_avg`` and ``exp_avg_sq`` are float32 tensors or
     :class:`Moment8`; 16-bit parameters need float32 ``masters``, which take the step and
-    are rounded into the parameters. ``step`` counts from 1. ``seed`` is that of the random
+    are rounded into the parameters. ``step`` counts from 1. ``eps`` below 1e-19 counts as that.
+    ``seed`` is that of the random
     rounding of 8-bit moments; ``(seed, step)`` repeated gives the same bits.
 
     With ``max_norm`` the gradients are scaled by ``min(1, max_norm / (norm + 1e-6))`` and

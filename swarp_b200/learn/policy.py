@@ -231,7 +231,7 @@ def policy_loss(
     constants. As with any autograd operation, none of them may be written to before the
     backward has run: that raises an error.
 
-    A masked row is never read and its gradient is exactly 0, whatever its inputs hold. A
+    A masked row adds nothing and its gradient is exactly 0, whatever its inputs hold. A
     logit of ``-inf`` is a token that cannot be chosen; a row of nothing else has ``logp``
     ``-inf``, entropy 0 and no loss or gradient, but counts in the mean. A token outside
     ``[0, V)`` makes the loss NaN. With no row admitted the loss is 0.
