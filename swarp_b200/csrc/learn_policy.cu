@@ -409,10 +409,13 @@ __device__ __forceinline__ float logp_of(float z, float m, float log2s) {
 // p with its sums on the maximum `top`, in place of its own; a rest is exchanged with the
 // maximum that it belongs to
 __device__ __forceinline__ void onto(Part& p, float top) {
-  const float d = max_nan(ordinary(top) && ordinary(p.m)
-                              ? __fsub_rn(scaled(p.m), scaled(top))
-                              : (p.m - origin(top)) * kLog2e + (rest(top) - rest(p.m)),
-                          -1e4f);
+  float d = __fsub_rn(scaled(p.m), scaled(top));
+  // far enough below an ordinary maximum (an empty part among them) nothing remains either way
+  if (!(ordinary(top) && (ordinary(p.m) || p.m < -1e6f))) {
+    asm volatile("");  // a branch, seldom taken, and no selection
+    d = (p.m - origin(top)) * kLog2e + (rest(top) - rest(p.m));
+  }
+  d = max_nan(d, -1e4f);
   const float f = exp2_fast(d);
   p.t = fmaf(p.s, d, p.t) * f;
   p.s *= f;
