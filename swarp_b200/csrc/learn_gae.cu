@@ -182,8 +182,10 @@ __global__ void __launch_bounds__(kColumnThreads)
 }
 
 // ------------------------------------------------------------------- few columns
-// (32,768 steps of six columns: 4 + 6 us, the latency of a few dependent loads each; threads of
-// their own took 6.3 ms, one for each column.) The steps are cut into segments, one per CTA, and a segment into runs of kRun steps, one
+// (32,768 steps of six columns: 4 + 6 us, most of it maps composed one after another: a thread of
+// the second kernel goes through its part of the later segments' and then through the n parts and
+// the runs after its own, n the CTA's runs of a column, 32 here and up to 256; the first kernel's
+// last step is such a chain too. Threads of their own took 6.3 ms, one for each column.) The steps are cut into segments, one per CTA, and a segment into runs of kRun steps, one
 // per thread. A thread forms its run's map from its own steps, the CTA composes the runs', and
 // the first kernel leaves the segment's map. The second kernel
 // composes the maps of the segments after its own, which is the advantage that follows it,

@@ -148,9 +148,9 @@ __global__ void __launch_bounds__(256) count_kernel(const uint8_t* mask, long lo
 // the first log2 R steps a lane hands half of its sums to its partner and keeps the other
 // half, so R sums cost R - 1 + log2(L / R) shuffles instead of R log2 L, and leave row
 // l / (L / R) with lane l. That lane then does the scalar part of its row, which would
-// otherwise cost every lane more than the row's own elements. Bound by its instructions: 200,000
-// rows of 128 floats take 46 us, 71% of the copy rate; of 100 bf16, which move one element at a
-// time, 69 us, 20%.
+// otherwise cost every lane more than the row's own elements. 200,000 rows of 128 floats take
+// 46 us, 71% of the copy rate, bound by 42 instructions an element (61% of the issue slots); of
+// 100 bf16 69 us, 20%, waiting for loads of two bytes.
 template <int L, int R, typename Op>
 __device__ __forceinline__ float reduce_rows(float (&v)[R], int lane, Op op) {
   int n = R;
@@ -532,7 +532,7 @@ constexpr int split_resident(int threads) { return 512 / split_block(threads); }
 // barrier would first wait for the gradient's stores. Each wait for parts has a limit. A warp that
 // comes to it sends no more, so all others come to theirs at the next row at the latest; what
 // they write from then on is NaN, and so is the loss.
-// 8192 rows of 131072 bf16 take 0.98 ms, 68% of the copy rate, 4096 of 32768 123 us, 68%;
+// 8192 rows of 131072 bf16 take 0.98 ms, 68% of the copy rate, 4096 of 32768 124 us, 67%;
 // about 18 instructions and two exponentials an element, which fill 55% of the issue slots and
 // 45% of the exponential unit, with 16 warps an SM to hide the rest.
 template <typename T, int THREADS, int C, bool GRAD>
@@ -821,7 +821,8 @@ __global__ void __launch_bounds__(split_block(THREADS), split_resident(THREADS))
 // waits for another's sums, and nothing is computed twice. E - 4 < V <= E. ROT: rows of an
 // even number of words would put many threads on one bank; they then start at different
 // places of their rows. 512,000 rows of 21 floats take 23 us, 70% of the copy rate (28
-// with a mask), bound by the copies' latency: six CTAs an SM, each waiting for its own.
+// with a mask): 40 instructions an element fill 71% of the issue slots, and a CTA that waits for
+// its copies, one tile at a time, has nothing else to do (six CTAs an SM).
 constexpr int kTileRows = 128;
 
 template <typename T, int E, bool ROT, bool GRAD>
@@ -949,7 +950,8 @@ __global__ void __launch_bounds__(kTileRows, 6) policy_tile_kernel(Args a) {
 
 // ------------------------------------------------------------- any row, any length
 // One CTA per row at a time, the row read three times (maximum, sums, gradient), the later
-// reads from L1 or L2.
+// reads from L1 or L2, element by element. 2048 rows of 151936 floats take 1.9 ms, 20% of the
+// copy rate (one read and one write), bound by the loads' latency.
 struct Block {
   float f[kLoopThreads / 32];
   float g[kLoopThreads / 32];
