@@ -42,7 +42,8 @@ class Moment8(NamedTuple):
 
     A code's value has an exponent and three bits of mantissa. Signed: a sign bit and seven
     bits ``f``, worth ``(f + 8 E - 112) << 20`` as float32 bits, 16 octaves. Unsigned: eight
-    bits, ``(f + 8 E - 247) << 20``, 32 octaves. ``f = 0`` is 0. A NaN or infinite gradient
+    bits, ``(f + 8 E - 247) << 20``, 32 octaves. ``f = 0`` is 0, and a signed ``f`` of 1 to 7 does
+    not occur. A NaN or infinite gradient
     makes its block's exponent 255, and the block's other elements lose their moments."""
 
     codes: torch.Tensor
@@ -243,7 +244,11 @@ class AdamW(torch.optim.Optimizer):
 
     ``state_bits`` 32 or 8; 16-bit parameters get a float32 master. ``max_norm`` clips the
     norm of all groups' gradients together; :attr:`grad_norm` is then that norm of the last
-    step (a device scalar). Parameters without a gradient are left out of a step."""
+    step (a device scalar). Parameters without a gradient are left out of a step.
+
+    A master is made at the parameter's first step and is what later steps update: after a
+    16-bit parameter has been changed from outside (weights loaded into the model, say),
+    set ``state[p]["master"]`` too."""
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 0.01, *, max_norm: float | None = None,
